@@ -168,6 +168,109 @@ int q35_attention_decode_paged(q35_context *ctx, const float *q, const float *ga
                                const int32_t *page_table, size_t max_pages,
                                const int32_t *seq_lens, size_t page_tokens, float *output,
                                size_t batch, int heads, int kv_heads, int head_dim, float scale);
+/* Attention of drafted trees over the paged cache (no reference counterpart:
+ * the reference checks drafted tokens one position at a time). Request b has
+ * context_lens[b] >= 0 committed tokens and the nodes node_start[b] ..
+ * node_start[b + 1] - 1, rows of q, gates and output ([rows][heads][head_dim];
+ * gates NULL: no gate). The K/V row of its node i lies at cache position
+ * context_lens[b] + i. A node sees every context row and each node j of its
+ * request whose bit is set in its mask (node_masks [rows][ceil(max_nodes / 64)]
+ * 64-bit words, bit j % 64 of word j / 64; bits past the request's nodes are
+ * ignored): output = softmax(scale q.k) v over those rows, times
+ * sigmoid(gate); a node that sees nothing, or whose scores are all -inf, gets
+ * zero. Infinite or NaN keys and values reach only the nodes that see their
+ * row (a key that is not finite may leave NaN in those).
+ *   head_dim 64, 128 or 256; heads a multiple of kv_heads; page_tokens a power
+ *   of two; at most 256 nodes a request; FP16 pools of total_pages pages;
+ *   16-byte aligned buffers; pools, table and masks are not written.
+ *   max_nodes, max_len: upper bounds of a request's nodes and of its context
+ *   plus nodes (max_len <= max_pages * page_tokens). They size the launch; the
+ *   nearer they are to the actual sizes, the fewer workgroups idle.
+ *   A request outside these bounds gets NaN in its rows (rows that node_start
+ *   does not place inside [0, rows) are left alone), and so does a node that
+ *   sees a row of a page outside [0, total_pages). Rows of no request are left
+ *   as they were.
+ * workspace: q35_attention_tree_workspace bytes, 256-byte aligned, not shared
+ * by calls that may overlap; NULL uses the context's own (refused while the
+ * stream is captured). The call reads nothing back and does not wait. */
+int q35_attention_tree_workspace(q35_context *ctx, size_t batch, size_t rows, size_t max_nodes,
+                                 size_t max_len, int heads, int kv_heads, int head_dim,
+                                 size_t *bytes);
+int q35_attention_tree_paged(q35_context *ctx, const float *q, const float *gates,
+                             const uint16_t *k_pool, const uint16_t *v_pool, size_t total_pages,
+                             const int32_t *page_table, size_t max_pages, size_t page_tokens,
+                             const int32_t *context_lens, const int32_t *node_start,
+                             const uint64_t *node_masks, float *output, size_t batch, size_t rows,
+                             size_t max_nodes, size_t max_len, int heads, int kv_heads,
+                             int head_dim, float scale, void *workspace, size_t workspace_bytes);
+/* The path of each request's tree that its sampled tokens accept (no reference
+ * counterpart). Node 0 (the pending token) is accepted; from an accepted node
+ * i the path goes on to its lowest child c (parents[c] == i, a node index of
+ * the request; children come after their parent) with draft_tokens[c] ==
+ * sampled_tokens[i], and ends where there is none. All arrays are [rows].
+ * path [batch][path_stride] receives the accepted nodes and -1 up to max_nodes
+ * entries, path_count their number, next_token the token sampled at the last
+ * one. A request without nodes, or outside max_nodes (at most 256) or rows,
+ * gets 0 nodes and token -1. */
+int q35_tree_accept(q35_context *ctx, const int32_t *node_start, const int32_t *parents,
+                    const int32_t *draft_tokens, const int32_t *sampled_tokens, int32_t *path,
+                    size_t path_stride, int32_t *path_count, int32_t *next_token, size_t batch,
+                    size_t rows, size_t max_nodes);
+
+/* ------------------------------------------------------------- sampling
+ * One token per row of device logits from given random numbers (the draw of
+ * sample_token_from_logits, src/runtime/layers.inl:491-600, on the device,
+ * with min-p and without its limit on the candidates). Per row:
+ *   penalty: a token with counts[row][token] > 0 has v / p for v > 0, else
+ *     v * p, where p > 1 (counts [rows][vocab], penalties [rows]);
+ *   order: larger values first, ties to the lower token; NaN counts as -inf;
+ *   weight of a token: exp((v - largest) / temperature); temperature <= 1e-6
+ *     or NaN takes the first token with probability 1;
+ *   top_k (0 or less, or all: off), top_p (>= 1: off; the shortest prefix that
+ *     holds top_p of the weight the first top_k tokens have), min_p (<= 0:
+ *     off; weights of at least min_p) each keep a prefix of the order, and the
+ *     shortest counts; the first token is always kept;
+ *   draw: the first token at which the running weight exceeds uniforms[row]
+ *     (0 <= u < 1) times the kept weight.
+ * Weights are summed as whole numbers of 2^-43, so a call gives the same
+ * tokens on every run. Tokens at -inf are never drawn; a row of nothing else
+ * gets token -1 and probability 0. out_probability (optional) is the token's
+ * weight over the kept weight. Row r of logits starts at r * stride; vocab is
+ * at most 2^20. Every option array may be NULL (off; temperature 1).
+ * workspace as for q35_attention_tree_paged (q35_sample_workspace bytes). */
+int q35_sample_workspace(q35_context *ctx, size_t rows, size_t vocab, size_t *bytes);
+int q35_sample_logits(q35_context *ctx, const float *logits, size_t stride, const int32_t *counts,
+                      const float *penalties, const float *temperatures, const int32_t *top_k,
+                      const float *top_p, const float *min_p, const float *uniforms, size_t rows,
+                      size_t vocab, int32_t *out_token, float *out_probability, void *workspace,
+                      size_t workspace_bytes);
+
+/* ------------------------------------------------- copies inside the cache
+ * K/V pools of `layers` layers, layer_stride elements apart, each
+ * [total_pages][page_tokens][row_elems] FP16 (row_elems = kv_heads * head_dim).
+ *
+ * q35_cache_copy_pages: rows [0, tokens[i]) of page src_pages[i] to page
+ * dst_pages[i] in every layer (tokens NULL: whole pages), KvPagesF16's copy on
+ * write (include/qwen35x/cpu/kv_pages.h:52-60) for many pages at once. The
+ * three arrays are HOST memory; a page written twice, or both read and
+ * written, is refused, as is one outside the pool. Under stream capture the
+ * pages become part of the graph. */
+int q35_cache_copy_pages(q35_context *ctx, uint16_t *k_pool, uint16_t *v_pool, size_t layers,
+                         size_t layer_stride, size_t total_pages, size_t page_tokens,
+                         size_t row_elems, const int32_t *src_pages, const int32_t *dst_pages,
+                         const int32_t *tokens, size_t count);
+/* q35_cache_compact_rows: for each request and j < path_count[b], in order,
+ * the cache row at position context_lens[b] + path[b][j] moves to position
+ * context_lens[b] + j (path as q35_tree_accept leaves it: path[j] >= j), in
+ * every layer. The arrays are DEVICE memory; a request whose path or pages are
+ * out of bounds is left as it is. The moved rows' pages must be the request's
+ * own. page_tokens is a power of two. */
+int q35_cache_compact_rows(q35_context *ctx, uint16_t *k_pool, uint16_t *v_pool, size_t layers,
+                           size_t layer_stride, size_t total_pages, size_t page_tokens,
+                           size_t row_elems, const int32_t *page_table, size_t max_pages,
+                           const int32_t *context_lens, const int32_t *path, size_t path_stride,
+                           const int32_t *path_count, size_t batch);
+
 /* attention_cache_store_f16, full_attention.h:22-26 (RNE, quiet NaN) */
 int q35_attention_cache_store_f16(q35_context *ctx, const float *input, uint16_t *output,
                                   size_t count);
@@ -299,6 +402,13 @@ int q35_page_alloc(q35_runtime *rt, int32_t *out_page);
 int q35_page_retain(q35_runtime *rt, int32_t page);
 int q35_page_release(q35_runtime *rt, int32_t page);
 int q35_page_copy(q35_runtime *rt, int32_t src_page, int32_t dst_page, int32_t tokens);
+/* Continuations of one request (no reference counterpart; several samples of a
+ * prompt): out_pages [children][count] receives the pages of each child. The
+ * `count` pages cover exactly `tokens` positions; full pages are shared
+ * (q35_page_retain), a partly filled last page is copied for every child. On
+ * an error nothing is retained or allocated. */
+int q35_page_fork(q35_runtime *rt, const int32_t *pages, size_t count, int32_t tokens, size_t children,
+                  int32_t *out_pages);
 int q35_page_refcount(q35_runtime *rt, int32_t page);
 int q35_runtime_free_pages(q35_runtime *rt);
 

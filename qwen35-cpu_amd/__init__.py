@@ -184,6 +184,16 @@ _SIGS = {
     "q35_attention_decode_paged": (c_int, [P, P, P, P, P, P, c_size_t, P, c_size_t, P, c_size_t, c_int,
                                            c_int, c_int, c_float]),
     "q35_attention_cache_store_f16": (c_int, [P, P, P, c_size_t]),
+    "q35_attention_tree_workspace": (c_int, [P, c_size_t, c_size_t, c_size_t, c_size_t, c_int, c_int, c_int,
+                                             POINTER(c_size_t)]),
+    "q35_attention_tree_paged": (c_int, [P, P, P, P, P, c_size_t, P, c_size_t, c_size_t, P, P, P, P, c_size_t, c_size_t,
+                                         c_size_t, c_size_t, c_int, c_int, c_int, c_float, P, c_size_t]),
+    "q35_tree_accept": (c_int, [P, P, P, P, P, P, c_size_t, P, P, c_size_t, c_size_t, c_size_t]),
+    "q35_sample_workspace": (c_int, [P, c_size_t, c_size_t, POINTER(c_size_t)]),
+    "q35_sample_logits": (c_int, [P, P, c_size_t, P, P, P, P, P, P, P, c_size_t, c_size_t, P, P, P, c_size_t]),
+    "q35_cache_copy_pages": (c_int, [P, P, P, c_size_t, c_size_t, c_size_t, c_size_t, c_size_t, P, P, P, c_size_t]),
+    "q35_cache_compact_rows": (c_int, [P, P, P, c_size_t, c_size_t, c_size_t, c_size_t, c_size_t, P, c_size_t, P, P,
+                                       c_size_t, P, c_size_t]),
     "q35_rms_norm_f32": (c_int, [P, P, P, P, c_size_t, c_size_t, c_float, c_float]),
     "q35_l2_normalize_f32": (c_int, [P, P, c_size_t, c_size_t, c_float, c_float]),
     "q35_causal_conv1d_silu_f32": (c_int, [P, P, c_size_t, P, c_size_t, P, P, c_size_t, c_size_t, c_size_t,
@@ -207,6 +217,7 @@ _SIGS = {
     "q35_page_retain": (c_int, [P, c_int32]),
     "q35_page_release": (c_int, [P, c_int32]),
     "q35_page_copy": (c_int, [P, c_int32, c_int32, c_int32]),
+    "q35_page_fork": (c_int, [P, P, c_size_t, c_int32, c_size_t, P]),
     "q35_page_refcount": (c_int, [P, c_int32]),
     "q35_runtime_free_pages": (c_int, [P]),
     "q35_runtime_step": (c_int, [P, POINTER(StepDesc), P, P]),
@@ -321,9 +332,10 @@ class DeviceArray:
 class Context:
     """One device, one stream (replaces the reference CpuExecutor)."""
 
-    def __init__(self, device: int = 0):
+    def __init__(self, device: int = 0, stream=None):
+        """stream: a hipStream_t (as an integer) to run on, None: one of its own."""
         h = c_void_p()
-        _check(lib.q35_context_create(device, None, ctypes.byref(h)), "context create")
+        _check(lib.q35_context_create(device, stream, ctypes.byref(h)), "context create")
         self.handle = h
 
     def device_info(self):
@@ -431,6 +443,79 @@ def attention_decode_paged(ctx, q, gates, k_pool, v_pool, page_table, max_pages,
     ctx.check(lib.q35_attention_decode_paged(ctx.handle, q.ptr, gates.ptr, k_pool.ptr, v_pool.ptr, page_table.ptr,
                                              max_pages, seq_lens.ptr, page_tokens, out.ptr, batch, heads, kv_heads,
                                              head_dim, scale), "attention_decode_paged")
+
+
+def _opt(a):
+    return a.ptr if a is not None else None
+
+
+def _workspace(workspace):
+    """A workspace buffer as its address and size (None: the context's own)."""
+    return (None, 0) if workspace is None else (workspace.ptr, workspace.nbytes)
+
+
+def attention_tree_workspace(ctx, batch, rows, max_nodes, max_len, heads, kv_heads, head_dim):
+    """Bytes of the workspace that attention_tree_paged needs for these sizes."""
+    n = c_size_t()
+    ctx.check(lib.q35_attention_tree_workspace(ctx.handle, batch, rows, max_nodes, max_len, heads, kv_heads, head_dim,
+                                               ctypes.byref(n)), "attention_tree_workspace")
+    return n.value
+
+
+def attention_tree_paged(ctx, q, gates, k_pool, v_pool, total_pages, page_table, max_pages, page_tokens, context_lens,
+                         node_start, node_masks, out, batch, rows, max_nodes, max_len, heads, kv_heads, head_dim, scale,
+                         workspace=None):
+    """Attention of every request's tree of drafted nodes over its cached context and the nodes its mask names."""
+    work, size = _workspace(workspace)
+    ctx.check(lib.q35_attention_tree_paged(ctx.handle, q.ptr, _opt(gates), k_pool.ptr, v_pool.ptr, total_pages,
+                                           page_table.ptr, max_pages, page_tokens, context_lens.ptr, node_start.ptr,
+                                           node_masks.ptr, out.ptr, batch, rows, max_nodes, max_len, heads, kv_heads,
+                                           head_dim, scale, work, size), "attention_tree_paged")
+
+
+def tree_accept(ctx, node_start, parents, draft_tokens, sampled_tokens, path, path_stride, path_count, next_token, batch,
+                rows, max_nodes):
+    """The path of each request's tree whose drafted tokens are the ones sampled at their parents."""
+    ctx.check(lib.q35_tree_accept(ctx.handle, node_start.ptr, parents.ptr, draft_tokens.ptr, sampled_tokens.ptr, path.ptr,
+                                  path_stride, path_count.ptr, next_token.ptr, batch, rows, max_nodes), "tree_accept")
+
+
+def sample_workspace(ctx, rows, vocab):
+    """Bytes of the workspace that sample_logits needs for these sizes."""
+    n = c_size_t()
+    ctx.check(lib.q35_sample_workspace(ctx.handle, rows, vocab, ctypes.byref(n)), "sample_workspace")
+    return n.value
+
+
+def sample_logits(ctx, logits, stride, counts, penalties, temperatures, top_k, top_p, min_p, uniforms, rows, vocab,
+                  out_token, out_probability=None, workspace=None):
+    """One token per row from given random numbers; each option is a [rows] buffer or None (off)."""
+    work, size = _workspace(workspace)
+    ctx.check(lib.q35_sample_logits(ctx.handle, logits.ptr, stride, _opt(counts), _opt(penalties), _opt(temperatures),
+                                    _opt(top_k), _opt(top_p), _opt(min_p), uniforms.ptr, rows, vocab, out_token.ptr,
+                                    _opt(out_probability), work, size), "sample_logits")
+
+
+def _page_list(a):
+    return np.ascontiguousarray(a, np.int32)
+
+
+def cache_copy_pages(ctx, k_pool, v_pool, layers, layer_stride, total_pages, page_tokens, row_elems, src, dst, tokens=None):
+    """Copies (the first tokens[i] rows of) page src[i] to page dst[i] in every layer; src, dst, tokens on the host."""
+    src, dst = _page_list(src), _page_list(dst)
+    tokens = _page_list(tokens) if tokens is not None else None
+    if src.ndim != 1 or src.shape != dst.shape or (tokens is not None and tokens.shape != src.shape):
+        raise ValueError("cache_copy_pages: src, dst and tokens are lists of one length")
+    ctx.check(lib.q35_cache_copy_pages(ctx.handle, k_pool.ptr, v_pool.ptr, layers, layer_stride, total_pages, page_tokens,
+                                       row_elems, _ptr(src), _ptr(dst), _ptr(tokens), src.size), "cache_copy_pages")
+
+
+def cache_compact_rows(ctx, k_pool, v_pool, layers, layer_stride, total_pages, page_tokens, row_elems, page_table,
+                       max_pages, context_lens, path, path_stride, path_count, batch):
+    """Moves the cache rows of accepted nodes together behind each request's context, in every layer."""
+    ctx.check(lib.q35_cache_compact_rows(ctx.handle, k_pool.ptr, v_pool.ptr, layers, layer_stride, total_pages, page_tokens,
+                                         row_elems, page_table.ptr, max_pages, context_lens.ptr, path.ptr, path_stride,
+                                         path_count.ptr, batch), "cache_compact_rows")
 
 
 def attention_cache_store_f16(ctx, x, out, count):
@@ -576,6 +661,18 @@ class Runtime(_Profiled):
 
     def page_release(self, page):
         self.ctx.check(lib.q35_page_release(self.handle, page), "page release")
+
+    def page_copy(self, src, dst, tokens):
+        """The first `tokens` rows of page src into page dst, every layer (copy on write)."""
+        self.ctx.check(lib.q35_page_copy(self.handle, src, dst, tokens), "page copy")
+
+    def page_fork(self, pages, tokens, children=1):
+        """Page lists [children][len(pages)] of continuations of `tokens` positions: full pages shared, a partly
+        filled last page copied for each."""
+        pages = np.ascontiguousarray(pages, np.int32)
+        out = np.zeros((children, pages.size), np.int32)
+        self.ctx.check(lib.q35_page_fork(self.handle, _ptr(pages), pages.size, tokens, children, _ptr(out)), "page fork")
+        return out
 
     def step(self, slots, positions, tokens, page_table, count_input=None, penalties=None, logits=False):
         slots = np.ascontiguousarray(slots, np.int32)

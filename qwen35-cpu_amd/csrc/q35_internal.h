@@ -21,6 +21,8 @@ struct Context {
   std::string arch;
   std::string error;
   hipEvent_t t0 = nullptr, t1 = nullptr;
+  void *work = nullptr;  // grow-only workspace of the calls that are given none of their own
+  size_t work_bytes = 0;
   int32_t *host_lens = nullptr;  // pinned, grow-only: context lengths read back by the attention entry point
   size_t host_lens_capacity = 0;
 };
@@ -464,6 +466,79 @@ hipError_t launch_attention(const AttnArgs &a, hipStream_t stream);
 constexpr int kAttnChunkTokens = 64;
 hipError_t launch_attention_merge(const AttnArgs &a, const float *gates, float *out, uint64_t *codes,
                                   float *scales, uint64_t seed, hipStream_t stream);
+
+// Attention of drafted trees (tree.hip): request b's nodes are the rows
+// node_start[b] .. node_start[b + 1] - 1 of q / gates / out, their K/V rows lie
+// behind its context_lens[b] context rows; masks [rows][mask_words].
+constexpr int kMaxTreeNodes = 256;
+struct TreeArgs {
+  const float *q = nullptr, *gates = nullptr;  // [rows][heads][head_dim]; gates optional
+  const uint16_t *k_pool = nullptr, *v_pool = nullptr;
+  const int32_t *page_table = nullptr;  // [batch][max_pages]
+  int total_pages = 0, max_pages = 0, page_shift = 0;
+  const int32_t *context_lens = nullptr, *node_start = nullptr;
+  const uint64_t *masks = nullptr;
+  int mask_words = 1;
+  float *out = nullptr;
+  int batch = 0, rows = 0, max_nodes = 0, max_len = 0, heads = 0, kv_heads = 0, head_dim = 0;
+  float scale = 1.0F;
+  int split_tokens = 0, splits = 1;              // cache rows per range, ranges (tree_plan)
+  float *part_o = nullptr, *part_ml = nullptr;   // splits > 1: [split][rows][heads][head_dim], [..][2] (max, sum)
+};
+void tree_plan(int batch, int max_nodes, int max_len, int heads, int kv_heads, int cu_count, int *split_tokens, int *splits);
+hipError_t launch_tree_attention(const TreeArgs &a, hipStream_t stream);
+
+struct AcceptArgs {
+  const int32_t *node_start = nullptr, *parents = nullptr, *draft_tokens = nullptr, *sampled_tokens = nullptr;
+  int32_t *path = nullptr, *path_count = nullptr, *next_token = nullptr;
+  int path_stride = 0, batch = 0, rows = 0, max_nodes = 0;
+};
+hipError_t launch_tree_accept(const AcceptArgs &a, hipStream_t stream);
+
+// Sampling with given random numbers (draw.hip). Per-row options are optional
+// (NULL: off); at most kDrawMaxVocab tokens.
+constexpr int kDrawMaxVocab = 1 << 20;
+struct DrawArgs {
+  const float *logits = nullptr;  // [rows][stride]
+  size_t stride = 0;
+  const int32_t *counts = nullptr;  // [rows][vocab]
+  const float *penalties = nullptr, *temperatures = nullptr;
+  const int32_t *top_k = nullptr;
+  const float *top_p = nullptr, *min_p = nullptr, *uniforms = nullptr;
+  int rows = 0, vocab = 0;
+  int32_t *out_token = nullptr;
+  float *out_probability = nullptr;
+};
+struct DrawScratch {  // per row and slice
+  int slices = 0;
+  unsigned long long *mass = nullptr, *list = nullptr;
+  uint16_t *ends = nullptr;
+  float *top = nullptr;
+};
+size_t draw_scratch_bytes(int rows, int vocab);
+hipError_t launch_draw(const DrawArgs &a, void *scratch, hipStream_t stream);
+
+// Copies inside the paged cache (cache.hip): pools of `layers` layers,
+// layer_stride elements apart, rows of row_elems binary16 values.
+struct PageCopyArgs {
+  uint16_t *k_pool = nullptr, *v_pool = nullptr;
+  int layers = 0, page_tokens = 0, row_elems = 0;
+  size_t layer_stride = 0;
+};
+constexpr int kCopyPairs = 256;  // pairs per launch, in the kernel's arguments (3 KiB)
+struct PagePairs {
+  int32_t src[kCopyPairs], dst[kCopyPairs], tokens[kCopyPairs];
+};
+hipError_t launch_page_copy(const PageCopyArgs &a, const PagePairs &pairs, int count, hipStream_t stream);
+
+struct CompactArgs {
+  uint16_t *k_pool = nullptr, *v_pool = nullptr;
+  int layers = 0, row_elems = 0, total_pages = 0, max_pages = 0, page_shift = 0;
+  size_t layer_stride = 0;
+  const int32_t *page_table = nullptr, *context_lens = nullptr, *path = nullptr, *path_count = nullptr;
+  int path_stride = 0, batch = 0;
+};
+hipError_t launch_row_compact(const CompactArgs &a, hipStream_t stream);
 
 // Elementwise / small ops (kernel-level entries and the step)
 hipError_t launch_rms_norm(const float *x, const float *w, float *y, int rows, int width,

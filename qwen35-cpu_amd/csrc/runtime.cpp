@@ -113,6 +113,7 @@ extern "C" void q35_context_destroy(q35_context *ctx) {
   (void)hipEventDestroy(ctx->t0);
   (void)hipEventDestroy(ctx->t1);
   if (ctx->host_lens != nullptr) (void)hipHostFree(ctx->host_lens);
+  if (ctx->work != nullptr) (void)hipFree(ctx->work);
   if (ctx->own_stream) (void)hipStreamDestroy(ctx->stream);
   delete ctx;
 }

@@ -147,4 +147,7 @@ int runtime_enqueue_step(q35_runtime *rt, const StepShape &shape, bool want_logi
 // Algorithmic HBM bytes of one GEMM launch: packed weights, A16 codes and
 // scales of every token, FP32 outputs (and the residual read when fused).
 double gemm_algorithmic_bytes(int rows, int nb, int tokens, bool stores, bool residual);
+// Page copies of checked pairs (drafted.cpp): tokens NULL copies whole pages.
+int copy_pages(q35_context *ctx, const PageCopyArgs &a, const int32_t *src, const int32_t *dst, const int32_t *tokens,
+               size_t count);
 }

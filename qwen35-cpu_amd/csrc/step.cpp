@@ -7,6 +7,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstring>
+#include <limits>
 #include <new>
 #include <string>
 #include <vector>
@@ -592,21 +593,71 @@ extern "C" int q35_page_refcount(q35_runtime *rt, int32_t p) {
 extern "C" int q35_runtime_free_pages(q35_runtime *rt) {
   return rt ? static_cast<int>(rt->free_pages.size()) : -1;
 }
+static PageCopyArgs page_copy_args(q35_runtime *rt) {
+  PageCopyArgs a;
+  a.k_pool = rt->k_pool;
+  a.v_pool = rt->v_pool;
+  a.layers = rt->model->n_full;
+  a.page_tokens = rt->cfg.page_tokens;
+  a.row_elems = rt->model->d.n_kv_heads * rt->model->d.head_dim;
+  a.layer_stride = rt->layer_pool_elems;
+  return a;
+}
 // Copy-on-write: the first `tokens` rows of src into dst, every full layer
 // (KvPagesF16::append on a shared tail page, kv_pages.h:52-60).
 extern "C" int q35_page_copy(q35_runtime *rt, int32_t src, int32_t dst, int32_t tokens) {
   if (rt == nullptr || src < 0 || dst < 0 || src >= rt->cfg.total_pages || dst >= rt->cfg.total_pages ||
       tokens < 0 || tokens > rt->cfg.page_tokens)
     return Q35_ERR_INVALID;
-  const size_t kvw = static_cast<size_t>(rt->model->d.n_kv_heads) * rt->model->d.head_dim;
-  const size_t page_elems = static_cast<size_t>(rt->cfg.page_tokens) * kvw;
-  const size_t bytes = static_cast<size_t>(tokens) * kvw * 2;
-  for (int l = 0; l < rt->model->n_full; ++l) {
-    const size_t base = l * rt->layer_pool_elems;
-    Q35_HIP_TRY(rt->ctx, hipMemcpyAsync(rt->k_pool + base + dst * page_elems, rt->k_pool + base + src * page_elems,
-                                        bytes, hipMemcpyDeviceToDevice, rt->ctx->stream));
-    Q35_HIP_TRY(rt->ctx, hipMemcpyAsync(rt->v_pool + base + dst * page_elems, rt->v_pool + base + src * page_elems,
-                                        bytes, hipMemcpyDeviceToDevice, rt->ctx->stream));
+  if (src == dst || rt->model->n_full == 0) return Q35_OK;
+  return copy_pages(static_cast<q35_context *>(rt->ctx), page_copy_args(rt), &src, &dst, &tokens, 1);
+}
+
+// `children` continuations of the same positions: they share the full pages
+// (one more holder each) and get copies of a partly filled last page, which
+// each will append to.
+extern "C" int q35_page_fork(q35_runtime *rt, const int32_t *pages, size_t count, int32_t tokens, size_t children,
+                             int32_t *out_pages) {
+  if (rt == nullptr) return Q35_ERR_INVALID;
+  Context *ctx = rt->ctx;
+  const int32_t page = rt->cfg.page_tokens;
+  if (tokens < 0 || count != (static_cast<size_t>(tokens) + page - 1) / page || (count > 0 && pages == nullptr) ||
+      (count > 0 && children > 0 && out_pages == nullptr))
+    return set_error(ctx, Q35_ERR_INVALID, "page fork: the pages must be those that cover the tokens");
+  if (count == 0 || children == 0) return Q35_OK;
+  const int32_t rest = tokens % page;
+  const size_t full = rest != 0 ? count - 1 : count;
+  for (size_t i = 0; i < count; ++i)
+    if (pages[i] < 0 || pages[i] >= rt->cfg.total_pages || rt->page_ref[pages[i]] <= 0)
+      return set_error(ctx, Q35_ERR_STATE, "page fork: a page that is not allocated");
+  for (size_t i = 0; i < full; ++i)
+    if (children > static_cast<size_t>(std::numeric_limits<int>::max()) / 2 - rt->page_ref[pages[i]])
+      return set_error(ctx, Q35_ERR_UNSUPPORTED, "page fork: too many holders of a page");
+  if (rest != 0 && rt->free_pages.size() < children) return set_error(ctx, Q35_ERR_OOM, "KV page pool exhausted");
+  std::vector<int32_t> src, dst, used;
+  try {
+    if (rest != 0) {
+      src.assign(children, pages[full]);
+      used.assign(children, rest);
+      dst.resize(children);
+    }
+  } catch (const std::bad_alloc &) {
+    return Q35_ERR_OOM;
+  }
+  for (size_t c = 0; c < dst.size(); ++c) (void)q35_page_alloc(rt, &dst[c]);
+  if (!dst.empty() && rt->model->n_full > 0) {
+    const int st = copy_pages(static_cast<q35_context *>(rt->ctx), page_copy_args(rt), src.data(), dst.data(), used.data(), children);
+    if (st != Q35_OK) {
+      for (const int32_t p : dst) (void)q35_page_release(rt, p);
+      return st;
+    }
+  }
+  for (size_t c = 0; c < children; ++c) {
+    for (size_t i = 0; i < full; ++i) {
+      ++rt->page_ref[pages[i]];
+      out_pages[c * count + i] = pages[i];
+    }
+    if (rest != 0) out_pages[c * count + full] = dst[c];
   }
   return Q35_OK;
 }
