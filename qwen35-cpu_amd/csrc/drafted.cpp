@@ -73,8 +73,6 @@ int workspace_get(q35_context *ctx, void *given, size_t given_bytes, size_t need
   return Q35_OK;
 }
 
-size_t align256(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
-
 // The shape checks of the tree attention and its plan; 0 or an error status.
 int tree_check(q35_context *ctx, size_t batch, size_t rows, size_t max_nodes, size_t max_len, int heads, int kv_heads,
                int head_dim, TreeArgs *a) {
@@ -93,14 +91,8 @@ int tree_check(q35_context *ctx, size_t batch, size_t rows, size_t max_nodes, si
   a->heads = heads;
   a->kv_heads = kv_heads;
   a->head_dim = head_dim;
-  tree_plan(a->batch, a->max_nodes, a->max_len, heads, kv_heads, ctx->cu_count, &a->split_tokens, &a->splits);
+  a->groups = tree_groups(a->batch, a->max_nodes, a->max_len, heads, kv_heads, ctx->cu_count);
   return Q35_OK;
-}
-
-size_t tree_bytes(const TreeArgs &a) {
-  if (a.splits <= 1) return 0;
-  const size_t n = static_cast<size_t>(a.splits) * a.rows * a.heads;
-  return align256(n * a.head_dim * 4) + align256(n * 8);
 }
 
 int draw_check(q35_context *ctx, size_t rows, size_t vocab) {
@@ -151,7 +143,8 @@ extern "C" int q35_attention_tree_workspace(q35_context *ctx, size_t batch, size
     if (bytes == nullptr) return set_error(ctx, Q35_ERR_INVALID, "tree attention: no place for the size");
     TreeArgs a;
     const int st = tree_check(ctx, batch, rows, max_nodes, max_len, heads, kv_heads, head_dim, &a);
-    if (st == Q35_OK) *bytes = tree_bytes(a);
+    size_t marks = 0, part_o = 0, part_ml = 0;
+    if (st == Q35_OK) *bytes = tree_workspace_bytes(a, &marks, &part_o, &part_ml);
     return st;
   });
 }
@@ -181,7 +174,8 @@ extern "C" int q35_attention_tree_paged(q35_context *ctx, const float *q, const 
     if (!std::isfinite(scale)) return set_error(ctx, Q35_ERR_INVALID, "tree attention: scale is not finite");
     if (rows == 0) return Q35_OK;
     void *work = nullptr;
-    st = workspace_get(ctx, workspace, workspace_bytes, tree_bytes(a), &work);
+    size_t marks = 0, part_o = 0, part_ml = 0;
+    st = workspace_get(ctx, workspace, workspace_bytes, tree_workspace_bytes(a, &marks, &part_o, &part_ml), &work);
     if (st != Q35_OK) return st;
     a.q = q;
     a.gates = gates;
@@ -197,10 +191,10 @@ extern "C" int q35_attention_tree_paged(q35_context *ctx, const float *q, const 
     a.mask_words = (a.max_nodes + 63) / 64;
     a.out = output;
     a.scale = scale;
-    a.part_o = static_cast<float *>(work);
-    if (work != nullptr)
-      a.part_ml = reinterpret_cast<float *>(
-          static_cast<char *>(work) + align256(static_cast<size_t>(a.splits) * a.rows * a.heads * a.head_dim * 4));
+    a.first_units = static_cast<long long *>(work);
+    a.marks = reinterpret_cast<int32_t *>(static_cast<char *>(work) + marks);
+    a.part_o = reinterpret_cast<float *>(static_cast<char *>(work) + part_o);
+    a.part_ml = reinterpret_cast<float *>(static_cast<char *>(work) + part_ml);
     const hipError_t e = launch_tree_attention(a, ctx->stream);
     return e == hipSuccess ? Q35_OK : hip_error(ctx, e, "tree attention");
   });

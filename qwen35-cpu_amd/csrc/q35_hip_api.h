@@ -52,6 +52,33 @@ typedef float q35_f32x4 __attribute__((ext_vector_type(4)));
 typedef float q35_f32x2 __attribute__((ext_vector_type(2)));
 #define Q35_LOAD_NT(ptr) __builtin_nontemporal_load(ptr)
 #define Q35_STORE_NT(value, ptr) __builtin_nontemporal_store(value, ptr)
+// 16 bytes per lane straight from global memory to LDS: lane l's land at the
+// wave-uniform address `lds` + 16 l. Counted like a load (in order); nothing
+// waits for it but Q35_WAIT_VM and a barrier behind that.
+#define Q35_LOAD_LDS16(global, lds)                                                                  \
+  __builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) void *)(global),               \
+                                   (__attribute__((address_space(3))) void *)(lds), 16, 0, 0)
+// Transposing LDS read of binary16: in each group of 16 lanes, lane c supplies
+// the address of four values, which are columns 4 (c % 4) .. + 3 of row c / 4 of
+// a 4 x 16 block, and receives column c: rows 0 .. 3.
+typedef short q35_s16x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ q35_u32x2 q35_lds_read_tr16(const uint16_t *lds) {
+  return __builtin_bit_cast(
+      q35_u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) q35_s16x4 *)(lds)));
+}
+// The maximum over lanes l, l ^ 16, l ^ 32 and l ^ 48: two exchanges of rows and
+// halves between registers. (With both operands x, the swap leaves the even
+// rows in one and the odd rows in the other.)
+__device__ __forceinline__ float q35_max_rows(float x) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  const float y = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  const auto h = __builtin_amdgcn_permlane32_swap(__float_as_uint(y), __float_as_uint(y), false, false);
+  return fmaxf(__uint_as_float(h[0]), __uint_as_float(h[1]));
+}
+// 2^x, results below 2^-126 as 0 (v_exp_f32, 1 ulp).
+#define Q35_EXP2(x) __builtin_amdgcn_exp2f(x)
+// Waits until at most n (a constant) of the wavefront's loads are outstanding.
+#define Q35_WAIT_VM(n) __builtin_amdgcn_s_waitcnt(((n) & 15) | (((n) >> 4) << 14) | 0x0f70)
 #endif
 
 #ifndef Q35_HOST_EMULATION

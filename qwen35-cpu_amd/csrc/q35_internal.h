@@ -482,10 +482,14 @@ struct TreeArgs {
   float *out = nullptr;
   int batch = 0, rows = 0, max_nodes = 0, max_len = 0, heads = 0, kv_heads = 0, head_dim = 0;
   float scale = 1.0F;
-  int split_tokens = 0, splits = 1;              // cache rows per range, ranges (tree_plan)
-  float *part_o = nullptr, *part_ml = nullptr;   // splits > 1: [split][rows][heads][head_dim], [..][2] (max, sum)
+  int groups = 1;                                // workgroups (tree_groups)
+  long long *first_units = nullptr;              // [batch + 1] work units before each request
+  int32_t *marks = nullptr;                      // [batch] values that are not finite in node rows
+  float *part_o = nullptr, *part_ml = nullptr;   // two parts per workgroup: [..][head_dim], [..][2] (max, sum)
 };
-void tree_plan(int batch, int max_nodes, int max_len, int heads, int kv_heads, int cu_count, int *split_tokens, int *splits);
+int tree_groups(int batch, int max_nodes, int max_len, int heads, int kv_heads, int cu_count);
+// Workspace bytes, and where marks, part_o and part_ml lie in it (first_units at 0).
+size_t tree_workspace_bytes(const TreeArgs &a, size_t *marks, size_t *part_o, size_t *part_ml);
 hipError_t launch_tree_attention(const TreeArgs &a, hipStream_t stream);
 
 struct AcceptArgs {

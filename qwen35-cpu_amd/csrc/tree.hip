@@ -14,21 +14,37 @@
 namespace q35 {
 namespace {
 
-constexpr int kTileTokens = 32;   // cache rows per tile
-constexpr int kBlockVectors = 32; // query vectors (node, head) per workgroup
-constexpr int kTreeWaves = 4;
-// Probabilities enter the second product times 2^14, as two binary16 operands
-// (22 bits): binary16 then holds them down to 2^-38 of the largest.
-constexpr float kProbUnit = 16384.0F;
+constexpr int kTileTokens = 32;    // cache rows per tile
+constexpr int kStageTokens = 64;   // cache rows per stage: two tiles
+constexpr int kGroupVectors = 16;  // query vectors (node, head) per wavefront
+constexpr int kTreeWaves = 8;
+constexpr int kBlockVectors = kTreeWaves * kGroupVectors;  // query vectors per item
+// Probabilities are taken relative to the running maximum less 14 binades: as
+// two binary16 operands (22 bits) they then reach down to 2^-38 of the largest.
+constexpr float kProbBinades = 14.0F;
 
-// Products of 32 cache rows and 32 query vectors on v_mfma_f32_32x32x16_f16,
-// with the cache as the A operand in both: S^T[t][m] = sum_d k[t][d] q[m][d]
-// and O^T[d][m] = sum_t v[t][d] p[m][t]. Lane l holds column m = l % 32 of
-// either result, rows 8(i / 4) + 4(l / 32) + i % 4 in its 16 registers, so the
-// softmax of a vector stays in two lanes (l and l ^ 32) and the probabilities
-// are the second product's B operand as they lie: k slot (l / 32, i) of step
-// ks stands for token 16 ks + 8(i / 4) + 4(l / 32) + i % 4 on both sides.
-__device__ __forceinline__ int slot_token(int i, int half) { return 8 * (i >> 2) + 4 * half + (i & 3); }
+// Products of cache rows and 16 query vectors on v_mfma_f32_16x16x32_f16, with
+// the cache as the A operand in both: S^T[t][m] = sum_d k[t][d] q[m][d] and
+// O^T[d][m] = sum_t v[t][d] p[m][t]. Lane l holds column m = l % 16 of either
+// result, rows 4(l / 16) + i in its 4 registers, so a vector's softmax stays in
+// four lanes and the probabilities of a tile's two score products are the
+// second product's B operand as they lie: k slot (l / 16, i) stands for the
+// tile's token 16(i / 4) + 4(l / 16) + i % 4 on both sides.
+__device__ __forceinline__ int slot_token(int i, int quad) { return 16 * (i >> 2) + 4 * quad + (i & 3); }
+
+// 2^(s * scale - ref), the product rounded on its own: the largest score then
+// meets its own value in ref (a contracted difference would leave the rounding
+// of ref, which an infinite weight could come of where scores are huge).
+__device__ __forceinline__ float score_weight(float s, float scale, float ref) {
+#pragma clang fp contract(off)
+  const float x = s * scale;
+  return Q35_EXP2(x - ref);
+}
+__device__ __forceinline__ float score_ref(float s, float scale) {
+#pragma clang fp contract(off)
+  const float x = s * scale;
+  return x - kProbBinades;
+}
 
 struct TreeRequest {
   int row0, nodes, context, len;  // first row, node rows, context rows, all rows
@@ -65,312 +81,463 @@ __device__ __forceinline__ uint32_t tree_visible(const uint64_t *words, int word
   return end - t < kTileTokens ? bits & ((1u << (end - t)) - 1u) : bits;
 }
 
-// DPL halfs of a cache row per lane, 32 lanes to a row
-template <int DPL>
-struct RowPiece;
-template <>
-struct RowPiece<8> {
-  typedef q35_u32x4 T;
-  static __device__ __forceinline__ uint32_t dword(const T &v, int i) { return v[i]; }
-  static __device__ __forceinline__ T zero() { return T{0u, 0u, 0u, 0u}; }
-};
-template <>
-struct RowPiece<4> {
-  typedef q35_u32x2 T;
-  static __device__ __forceinline__ uint32_t dword(const T &v, int i) { return v[i]; }
-  static __device__ __forceinline__ T zero() { return T{0u, 0u}; }
-};
-template <>
-struct RowPiece<2> {
-  typedef uint32_t T;
-  static __device__ __forceinline__ uint32_t dword(const T &v, int) { return v; }
-  static __device__ __forceinline__ T zero() { return 0u; }
-};
-
-// Whether either binary16 half of a dword is infinite or NaN.
-__device__ __forceinline__ bool half2_special(uint32_t w) {
-  return (w & 0x7c00u) == 0x7c00u || (w & 0x7c000000u) == 0x7c000000u;
-}
-
-// Normalisation and the sigmoid gate of four dims; a zero sum saw nothing.
-__device__ __forceinline__ q35_f32x4 tree_finish(q35_f32x4 o, float l, const float *gates) {
-  const float inv = 1.0F / (l == 0.0F ? 1.0F : l);
-  q35_f32x4 y = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
-  if (gates != nullptr) {
-    const q35_f32x4 x = *reinterpret_cast<const q35_f32x4 *>(gates);
+// N consecutive dims of an output (or of a part of one): normalised by the sum
+// l -- a zero sum saw nothing -- and gated.
+template <int N>
+__device__ __forceinline__ void tree_store(float *dst, const float y[N]) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) y[e] *= sigmoid_stable(x[e]);
+  for (int e = 0; e < N; e += 4) {
+    if constexpr (N >= 4) *reinterpret_cast<q35_f32x4 *>(dst + e) = q35_f32x4{y[e], y[e + 1], y[e + 2], y[e + 3]};
+    else if constexpr (N == 2) *reinterpret_cast<q35_f32x2 *>(dst) = q35_f32x2{y[0], y[1]};
+    else dst[0] = y[0];
   }
-  return y;
+}
+template <int N>
+__device__ __forceinline__ void tree_store(float *dst, const float y[N], float l, const float *gates) {
+  const float inv = 1.0F / (l == 0.0F ? 1.0F : l);
+  float z[N];
+#pragma unroll
+  for (int e = 0; e < N; ++e) z[e] = y[e] * inv;
+  if (gates != nullptr) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) z[e] *= sigmoid_stable(gates[e]);
+  }
+  tree_store<N>(dst, z);
 }
 
-// One workgroup per (range of cache rows, 32 query vectors of one KV head,
-// request): wavefront w takes the range's tiles w, w + 4, ... with a running
-// maximum and sum of its own, operands straight from the cache, and the four
-// are joined through LDS at the end.
+// The work is cut into units of one stage (64 cache rows) of one item (request,
+// KV head, block of up to 128 query vectors), items one after the other and the
+// stages of an item in order; request b has tree_units(b) of them. Workgroup w
+// of W takes units [w T / W, (w + 1) T / W) of all T, so ragged contexts leave
+// every CU the same share, whatever the host knew of the lengths. An item that
+// lies inside one workgroup's range is finished there; of the others each
+// workgroup leaves a part (maximum, sum, unnormalised output) in one of its two
+// places: the second where its range holds the item's first unit, else the
+// first (a range has at most one of each).
+__device__ __forceinline__ int item_blocks(const TreeArgs &a, const TreeRequest &r) {
+  return (r.nodes * (a.heads / a.kv_heads) + kBlockVectors - 1) / kBlockVectors;
+}
+__device__ __forceinline__ int item_stages(const TreeRequest &r) { return (r.len + kStageTokens - 1) / kStageTokens; }
+__device__ __forceinline__ long long tree_units(const TreeArgs &a, int b) {
+  const TreeRequest r = tree_request(a, b);
+  return static_cast<long long>(a.kv_heads) * item_blocks(a, r) * item_stages(r);
+}
+// W: the launched workgroups, or as many as there are units, so that no range
+// before the last is empty.
+__device__ __forceinline__ int unit_groups(const TreeArgs &a, long long total) {
+  return total < a.groups ? static_cast<int>(max(total, 1LL)) : a.groups;
+}
+__device__ __forceinline__ long long unit_begin(long long w, long long total, int groups) { return w * total / groups; }
+__device__ __forceinline__ int unit_group(long long unit, long long total, int groups) {
+  return static_cast<int>(((unit + 1) * groups - 1) / total);
+}
+
+// One workgroup of eight wavefronts. A stage's K and V rows go straight from
+// the cache to LDS (16 bytes a lane, one stage ahead of the products), each
+// read once for up to 128 vectors. With five to eight groups of 16 vectors each
+// wavefront has one and takes both tiles of a stage; with fewer, two wavefronts
+// share a group, a tile each, and are joined at the end. A wavefront keeps its
+// queries and its output in registers throughout, two wavefronts to a SIMD, so
+// that one's softmax runs beside the other's products. (Groups of 32 vectors
+// would read LDS half as often, but one wavefront then fills a SIMD's registers
+// and nothing runs beside it.)
+//
+// In LDS a K row's 16-byte pieces are rotated by xor with the row number, and a
+// V row's pairs of pieces, so that the lanes of an operand (16 rows' piece, or
+// pair) read distinct banks; the cache is read in the same order (whole rows,
+// permuted inside). The value operands, whose lanes need one dim of several
+// rows, come out of LDS by transposing reads.
 template <int HD>
-__global__ __launch_bounds__(64 * kTreeWaves) Q35_WAVES_PER_EU(1) void tree_attention_kernel(TreeArgs a) {
-  constexpr int DPL = HD / 32;    // dims of a value row per lane
-  constexpr int KS = HD / 16;     // 16-dim steps of the score product
-  constexpr int PART = HD / 4;    // dims joined per round
-  constexpr int STRIDE = PART + 4;
-  typedef typename RowPiece<DPL>::T Piece;
-  constexpr int JOIN = STRIDE > kTileTokens ? STRIDE : kTileTokens;  // floats per wavefront and vector
-  __shared__ __align__(16) float join[kTreeWaves * kBlockVectors * JOIN];
-  __shared__ float wave_max[kTreeWaves][kBlockVectors], wave_sum_[kTreeWaves][kBlockVectors];
-  const int sp = static_cast<int>(blockIdx.x), b = static_cast<int>(blockIdx.z);
-  const int g = static_cast<int>(blockIdx.y) % a.kv_heads, mb = static_cast<int>(blockIdx.y) / a.kv_heads;
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, col = lane & 31, half = lane >> 5;
-  const int qpk = a.heads / a.kv_heads;
-  const TreeRequest rq = tree_request(a, b);
-  if (!rq.valid) {
-    // refused on the device: NaN in the request's rows, where those are known
-    if (rq.rows_valid && sp == 0 && mb == 0)
-      for (int r = 0; r < rq.nodes; ++r)
-        for (int e = tid; e < qpk * HD; e += 64 * kTreeWaves)
-          a.out[(static_cast<size_t>(rq.row0 + r) * a.heads + g * qpk) * HD + e] = __uint_as_float(0x7fc00000u);
+__global__ __launch_bounds__(64 * kTreeWaves) Q35_WAVES_PER_EU(2) void tree_attention_kernel(TreeArgs a) {
+  constexpr int KS = HD / 32;    // 32-dim steps of the score product
+  constexpr int PIECES = HD / 8; // 16-byte pieces of a row
+  constexpr int NV = HD / 16;    // 16-dim value operands
+  constexpr int LOADS = kStageTokens * PIECES / (64 * kTreeWaves);  // pieces of K (and of V) per thread and stage
+  constexpr int BLOCK = kStageTokens * HD;  // halfs of a stage's K (or V)
+  // (One object: with several the compiler knows which of them the loads to LDS
+  // write, and waits for all of those before each read of it. The waits that
+  // are needed are the ones at the barriers.)
+  __shared__ struct __align__(1024) {
+    uint16_t cache[4 * BLOCK];       // [stage % 2][K, V][row][dim]
+    int rows[4][kStageTokens];       // cache rows of four stages (-1: none)
+    float stat[4][2][64];
+    long long scan[64 * kTreeWaves];
+    long long first_unit;
+    int first_request, marked;
+  } sh;
+  uint16_t *cache = sh.cache;
+  const int tid = threadIdx.x, wave = q35_uniform(tid >> 6), lane = tid & 63, col = lane & 15, quad = lane >> 4;
+  const int qpk = a.heads / a.kv_heads, w = static_cast<int>(blockIdx.x);
+  const size_t kvw = static_cast<size_t>(a.kv_heads) * HD;
+  const int shift = a.page_shift, pmask = (1 << shift) - 1;
+
+  // The workgroups behind those of the units mark each request with an infinite
+  // or NaN value in a node's row: products with probabilities of 0 would carry
+  // it to nodes that do not see the row, so the merge computes such requests
+  // anew.
+  if (w >= a.groups) {
+    for (int b = w - a.groups; b < a.batch; b += static_cast<int>(gridDim.x) - a.groups) {
+      const TreeRequest rq = tree_request(a, b);
+      if (tid == 0) sh.marked = 0;
+      __syncthreads();
+      const int32_t *table = a.page_table + static_cast<size_t>(b) * a.max_pages;
+      const int pieces = static_cast<int>(kvw / 8);
+      bool special = false;
+      for (int e = tid; rq.valid && e < rq.nodes * pieces; e += 64 * kTreeWaves) {
+        const int t = rq.context + e / pieces, page = table[t >> shift];
+        if (static_cast<unsigned>(page) >= static_cast<unsigned>(a.total_pages)) continue;
+        const q35_u32x4 v = *reinterpret_cast<const q35_u32x4 *>(
+            a.v_pool + static_cast<size_t>((page << shift) + (t & pmask)) * kvw + 8 * static_cast<size_t>(e % pieces));
+#pragma unroll
+        for (int d = 0; d < 4; ++d) special |= (v[d] & 0x7c00u) == 0x7c00u || (v[d] & 0x7c000000u) == 0x7c000000u;
+      }
+      if (special) sh.marked = 1;
+      __syncthreads();
+      if (tid == 0) a.marks[b] = sh.marked;
+      __syncthreads();
+    }
     return;
   }
-  const int vectors = rq.nodes * qpk, m0 = mb * kBlockVectors;
-  const int t0 = sp * a.split_tokens;
-  if (m0 >= vectors || t0 >= rq.len) return;  // whole workgroup
-  const int t1 = min(t0 + a.split_tokens, rq.len);
 
-  // the lane's query vector (spare lanes repeat the last one and see nothing)
-  const bool live = m0 + col < vectors;
-  const int m = min(m0 + col, vectors - 1), node = m / qpk, u = m - node * qpk;
-  const uint64_t *words = a.masks + static_cast<size_t>(rq.row0 + node) * a.mask_words;
-  q35_f16x8 qhi[KS], qlo[KS];
-  float sscale;
+  // running unit counts over the requests, a run of them per thread
+  const int run = (a.batch + 64 * kTreeWaves - 1) / (64 * kTreeWaves), b0 = min(tid * run, a.batch), b1 = min(b0 + run, a.batch);
+  long long mine = 0;
+  for (int b = b0; b < b1; ++b) mine += tree_units(a, b);
+  sh.scan[tid] = mine;
+  __syncthreads();
+  for (int d = 1; d < 64 * kTreeWaves; d <<= 1) {
+    const long long up = tid >= d ? sh.scan[tid - d] : 0;
+    __syncthreads();
+    sh.scan[tid] += up;
+    __syncthreads();
+  }
+  const long long total = sh.scan[64 * kTreeWaves - 1];
+  const int ranges = unit_groups(a, total);
+  const long long begin = unit_begin(min(w, ranges), total, ranges), end = unit_begin(min(w + 1, ranges), total, ranges);
   {
-    // the vector as two binary16 operands: 22 bits under its largest value,
-    // which a power of two brings to 2^8 (exact, and any fp32 size fits)
-    const float *src = a.q + (static_cast<size_t>(rq.row0 + node) * a.heads + g * qpk + u) * HD + 8 * half;
-    float x[KS][8], top = 0.0F;
-#pragma unroll
-    for (int kk = 0; kk < KS; ++kk) {
-      const q35_f32x4 lo = *reinterpret_cast<const q35_f32x4 *>(src + 16 * kk);
-      const q35_f32x4 hi = *reinterpret_cast<const q35_f32x4 *>(src + 16 * kk + 4);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        x[kk][i] = lo[i];
-        x[kk][4 + i] = hi[i];
-        top = fmaxf(top, fmaxf(fabsf(lo[i]), fabsf(hi[i])));
+    long long at = sh.scan[tid] - mine;
+    for (int b = b0; b < b1; ++b) {
+      const long long n = tree_units(a, b);
+      if (w == 0) a.first_units[b] = at;  // for the merge
+      if (begin >= at && begin < at + n) {
+        sh.first_request = b;
+        sh.first_unit = at;
       }
+      at += n;
     }
-    top = fmaxf(top, __shfl_xor(top, 32, 64));
-    int ex = static_cast<int>(__float_as_uint(top) >> 23);  // biased
-    ex = ex == 0 || ex == 255 ? 127 + 8 : max(ex, 20);
-    const float down = __uint_as_float(static_cast<uint32_t>(127 + 8 + 127 - ex) << 23);  // 2^(8 - exponent)
-    const float up = __uint_as_float(static_cast<uint32_t>(max(ex - 8, 1)) << 23);        // 2^(exponent - 8)
-    sscale = a.scale * 1.44269504088896341F * up;
-#pragma unroll
-    for (int kk = 0; kk < KS; ++kk) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[kk][i] *= down;
-      q35_split_f16(x[kk], qhi[kk], qlo[kk]);
-    }
-  }
-
-  const int shift = a.page_shift, pmask = (1 << shift) - 1;
-  const int32_t *table = a.page_table + static_cast<size_t>(b) * a.max_pages;
-  const size_t kvw = static_cast<size_t>(a.kv_heads) * HD;
-  const uint16_t *kcol = a.k_pool + static_cast<size_t>(g) * HD + 8 * half;
-  const uint16_t *vcol = a.v_pool + static_cast<size_t>(g) * HD + DPL * col;
-  // the cache row of token t + lane % 32 (rows past the range: the tile's
-  // first), and whether its page lies in the pool
-  auto cache_row = [&](int t, bool &ok) {
-    const int tt = t + col < t1 ? t + col : t;
-    const int page = table[tt >> shift];
-    ok = static_cast<unsigned>(page) < static_cast<unsigned>(a.total_pages);
-    return ((ok ? page : 0) << shift) + (tt & pmask);
-  };
-
-  q35_f32x16 acc[DPL];
-#pragma unroll
-  for (int j = 0; j < DPL; ++j)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) acc[j][i] = 0.0F;
-  float mx = -INFINITY, sum = 0.0F;  // the lane's vector; the sum over the lane's own tokens
-
-  for (int t = t0 + kTileTokens * wave; t < t1; t += kTileTokens * kTreeWaves) {
-    bool ok;
-    const int row = cache_row(t, ok);
-    const uint32_t lost = ~static_cast<uint32_t>(q35_ballot(ok));  // both halves hold the same 32 rows
-    const uint16_t *krow = kcol + static_cast<size_t>(row) * kvw;
-    q35_u32x4 kraw[KS];
-#pragma unroll
-    for (int kk = 0; kk < KS; ++kk) kraw[kk] = *reinterpret_cast<const q35_u32x4 *>(krow + 16 * kk);
-    Piece vraw[2][8];
-#pragma unroll
-    for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int vr = __shfl(row, slot_token(8 * ks + i, half), 64);
-        vraw[ks][i] = *reinterpret_cast<const Piece *>(vcol + static_cast<size_t>(vr) * kvw);
-      }
-    q35_f32x16 s;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) s[i] = 0.0F;
-#pragma unroll
-    for (int kk = 0; kk < KS; ++kk) {
-      const q35_f16x8 k = q35_f16x8_bits(kraw[kk]);
-      s = Q35_MFMA_F32_32X32X16_F16(k, qhi[kk], s);
-      s = Q35_MFMA_F32_32X32X16_F16(k, qlo[kk], s);
-    }
-    uint32_t seen = 0u;
-    if (live) seen = t + kTileTokens <= rq.context && t + kTileTokens <= t1 ? 0xffffffffu : tree_visible(words, a.mask_words, t, rq.context, t1);
-    float p[16], top = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int tok = slot_token(i, half);
-      float x = s[i] * sscale;
-      x = (lost >> tok) & 1u ? NAN : x;  // a page outside the pool
-      p[i] = (seen >> tok) & 1u ? x : -INFINITY;
-      top = fmaxf(top, p[i]);
-    }
-    top = fmaxf(top, __shfl_xor(top, 32, 64));
-    const float next = fmaxf(mx, top), base = next == -INFINITY ? 0.0F : next;
-    const float keep = mx == next ? 1.0F : exp2f(mx - base);  // 0 at the first seen row
-    float part = 0.0F;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      p[i] = exp2f(p[i] - base);
-      part += p[i];
-      p[i] *= kProbUnit;
-    }
-    sum = fmaf(sum, keep, part);
-    mx = next;
-    if (q35_ballot(keep != 1.0F) != 0ull) {
-#pragma unroll
-      for (int j = 0; j < DPL; ++j)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) acc[j][i] *= keep;
-    }
-    // Tiles with node rows: a value that is infinite or NaN reaches only the
-    // nodes that see its row (0 x inf would reach all), and spare slots hold 0.
-    bool special = false;
-    if (t + kTileTokens > rq.context) {
-#pragma unroll
-      for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int tt = t + slot_token(8 * ks + i, half);
-          if (tt >= t1) vraw[ks][i] = RowPiece<DPL>::zero();
-#pragma unroll
-          for (int d = 0; d < DPL / 2; ++d) special |= half2_special(RowPiece<DPL>::dword(vraw[ks][i], d));
-        }
-      special = q35_ballot(special) != 0ull;
-    }
-    if (!special) {
-#pragma unroll
-      for (int ks = 0; ks < 2; ++ks) {
-        q35_f16x8 phi, plo;
-        q35_split_f16(p + 8 * ks, phi, plo);
-#pragma unroll
-        for (int j = 0; j < DPL; ++j) {
-          const unsigned sel = (j & 1) ? 0x07060302u : 0x05040100u;
-          q35_u32x4 d;
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            d[e] = __builtin_amdgcn_perm(RowPiece<DPL>::dword(vraw[ks][2 * e + 1], j >> 1),
-                                         RowPiece<DPL>::dword(vraw[ks][2 * e], j >> 1), sel);
-          const q35_f16x8 v = q35_f16x8_bits(d);
-          acc[j] = Q35_MFMA_F32_32X32X16_F16(v, phi, acc[j]);
-          acc[j] = Q35_MFMA_F32_32X32X16_F16(v, plo, acc[j]);
-        }
-      }
-    } else {
-      float *pb = join + wave * kTileTokens * kBlockVectors;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) pb[slot_token(i, half) * kBlockVectors + col] = p[i];
-      wave_lds_sync();
-      for (int tok = 0; tok < min(kTileTokens, t1 - t); ++tok) {
-        const float pt = pb[tok * kBlockVectors + col];
-        const uint16_t *vrow = a.v_pool + static_cast<size_t>(__shfl(row, tok, 64)) * kvw + static_cast<size_t>(g) * HD;
-        if (!((seen >> tok) & 1u)) continue;
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-#pragma unroll
-          for (int j = 0; j < DPL; ++j)
-            acc[j][i] = fmaf(pt, half_bits_to_float(vrow[DPL * slot_token(i, half) + j]), acc[j][i]);
-      }
-      wave_lds_sync();
-    }
-  }
-
-  // the four wavefronts' parts of each vector
-  sum += __shfl_xor(sum, 32, 64);
-  if (half == 0) {
-    wave_max[wave][col] = mx;
-    wave_sum_[wave][col] = sum;
+    if (w == 0 && tid == 0) a.first_units[a.batch] = total;
   }
   __syncthreads();
-  float all = wave_max[0][col];
+  if (begin >= end) return;  // whole workgroup
+
+  int b = sh.first_request;
+  long long base = sh.first_unit;  // the request's first unit
+  for (long long unit = begin; unit < end;) {
+    const TreeRequest rq = tree_request(a, b);
+    const int stages = item_stages(rq), blocks = item_blocks(a, rq);
+    const long long request_units = static_cast<long long>(a.kv_heads) * blocks * stages;
+    if (unit >= base + request_units) {  // (a request without units among them)
+      base += request_units;
+      ++b;
+      continue;
+    }
+    const int item = static_cast<int>((unit - base) / stages), s0 = static_cast<int>((unit - base) - static_cast<long long>(item) * stages);
+    const int s1 = static_cast<int>(min(static_cast<long long>(stages), s0 + (end - unit)));
+    const int g = item / blocks, m0 = (item - g * blocks) * kBlockVectors;
+    unit += s1 - s0;
+
+    const int vectors = rq.nodes * qpk, groups = min(kTreeWaves, (vectors - m0 + kGroupVectors - 1) / kGroupVectors);
+    const bool shared = groups <= kTreeWaves / 2;  // two wavefronts to a group of vectors
+    const int group = shared ? wave & (kTreeWaves / 2 - 1) : wave, part = shared ? wave / (kTreeWaves / 2) : 0;
+    const bool active = group < groups;
+    const int mg = m0 + kGroupVectors * group;
+
+    const int32_t *table = a.page_table + static_cast<size_t>(b) * a.max_pages;
+    // token `tid` of stage s (tokens past the request: the stage's first), its
+    // page, and from that its cache row
+    auto stage_token = [&](int s) {
+      const int t = kStageTokens * min(s, s1 - 1);
+      return t + tid < rq.len ? t + tid : t;
+    };
+    auto stage_page = [&](int s) { return table[stage_token(s) >> shift]; };
+    auto stage_row = [&](int s, int page) {
+      return static_cast<unsigned>(page) < static_cast<unsigned>(a.total_pages) ? (page << shift) + (stage_token(s) & pmask) : -1;
+    };
+    auto issue = [&](int s) {
+      const int *at = sh.rows[s & 3];
+      const uint16_t *kp = a.k_pool + static_cast<size_t>(g) * HD, *vp = a.v_pool + static_cast<size_t>(g) * HD;
 #pragma unroll
-  for (int w = 1; w < kTreeWaves; ++w) all = fmaxf(all, wave_max[w][col]);
-  const float weight = exp2f(mx - (all == -INFINITY ? 0.0F : all)) * (1.0F / kProbUnit);
+      for (int i = 0; i < LOADS; ++i) {
+        const int e = i * 64 * kTreeWaves + tid, r = e / PIECES, slot = e % PIECES;
+        const size_t row = static_cast<size_t>(max(at[r], 0)) * kvw;
+        uint16_t *to = cache + (s & 1) * 2 * BLOCK + 8 * (i * 64 * kTreeWaves + 64 * wave);
+        Q35_LOAD_LDS16(kp + row + 8 * (slot ^ (r & (PIECES - 1))), to);
+        Q35_LOAD_LDS16(vp + row + 8 * (slot ^ (2 * r & (PIECES - 1))), to + BLOCK);
+      }
+    };
+    if (tid < kStageTokens) {
+      const int page0 = stage_page(s0), page1 = stage_page(s0 + 1);
+      sh.rows[s0 & 3][tid] = stage_row(s0, page0);
+      sh.rows[(s0 + 1) & 3][tid] = stage_row(s0 + 1, page1);
+    }
+    int following = tid < kStageTokens ? stage_page(s0 + 2) : 0;
+    lds_barrier();
+    issue(s0);
+
+    // the lane's query vector (spare lanes repeat the last one and store nothing)
+    const bool live = mg + col < vectors;
+    const int m = min(mg + col, vectors - 1), node = m / qpk, u = m - node * qpk;
+    const size_t head = static_cast<size_t>(rq.row0 + node) * a.heads + g * qpk + u;
+    const uint64_t *words = a.masks + static_cast<size_t>(rq.row0 + node) * a.mask_words;
+    q35_f16x8 qhi[KS], qlo[KS];
+    float sscale;
+    {
+      // the vector as two binary16 operands: 22 bits under its largest value,
+      // which a power of two brings to 2^8 (exact, and any fp32 size fits)
+      // (read twice, for the maximum and for the operands: the vector itself
+      // would take another 64 registers)
+      const float *src = a.q + head * HD + 8 * quad;
+      float top = 0.0F;
 #pragma unroll
-  for (int part = 0; part < 4; ++part) {
-    if (part > 0) __syncthreads();  // the last round's sums are read
-    float *mine = join + (wave * kBlockVectors + col) * STRIDE;
+      for (int kk = 0; kk < KS; ++kk) {
+        const q35_f32x4 lo = *reinterpret_cast<const q35_f32x4 *>(src + 32 * kk);
+        const q35_f32x4 hi = *reinterpret_cast<const q35_f32x4 *>(src + 32 * kk + 4);
 #pragma unroll
-    for (int ii = 0; ii < 4; ++ii)
+        for (int i = 0; i < 4; ++i) top = fmaxf(top, fmaxf(fabsf(lo[i]), fabsf(hi[i])));
+      }
+      q35_compiler_fence();
+      top = q35_max_rows(top);
+      int ex = static_cast<int>(__float_as_uint(top) >> 23);  // biased
+      ex = ex == 0 || ex == 255 ? 127 + 8 : max(ex, 20);
+      float down = __uint_as_float(static_cast<uint32_t>(127 + 8 + 127 - ex) << 23);  // 2^(8 - exponent)
+      const float up = __uint_as_float(static_cast<uint32_t>(max(ex - 8, 1)) << 23);        // 2^(exponent - 8)
+      sscale = fabsf(a.scale) * 1.44269504088896341F * up;
+      if (a.scale < 0.0F) down = -down;  // the scores' order is then that of the products
 #pragma unroll
-      for (int j = 0; j < DPL; ++j) mine[DPL * (4 * half + ii) + j] = acc[j][4 * part + ii] * weight;
-    __syncthreads();
-    for (int e = tid; e < kBlockVectors * PART / 4; e += 64 * kTreeWaves) {
-      const int v = e / (PART / 4), d = 4 * (e % (PART / 4));
-      if (m0 + v >= vectors) continue;
-      q35_f32x4 o = *reinterpret_cast<const q35_f32x4 *>(join + v * STRIDE + d);
+      for (int kk = 0; kk < KS; ++kk) {
+        const q35_f32x4 lo = *reinterpret_cast<const q35_f32x4 *>(src + 32 * kk);
+        const q35_f32x4 hi = *reinterpret_cast<const q35_f32x4 *>(src + 32 * kk + 4);
+        float x[8];
 #pragma unroll
-      for (int w = 1; w < kTreeWaves; ++w)
-        o += *reinterpret_cast<const q35_f32x4 *>(join + (w * kBlockVectors + v) * STRIDE + d);
-      float top = wave_max[0][v];
-#pragma unroll
-      for (int w = 1; w < kTreeWaves; ++w) top = fmaxf(top, wave_max[w][v]);
-      const float base = top == -INFINITY ? 0.0F : top;
-      float l = 0.0F;
-#pragma unroll
-      for (int w = 0; w < kTreeWaves; ++w) l = fmaf(wave_sum_[w][v], exp2f(wave_max[w][v] - base), l);
-      const int vn = (m0 + v) / qpk, vu = (m0 + v) - vn * qpk;
-      const size_t head = static_cast<size_t>(rq.row0 + vn) * a.heads + g * qpk + vu;
-      const int dim = PART * part + d;
-      if (a.splits > 1) {
-        const size_t at = static_cast<size_t>(sp) * a.rows * a.heads + head;
-        *reinterpret_cast<q35_f32x4 *>(a.part_o + at * HD + dim) = o;
-        if (dim == 0) *reinterpret_cast<q35_f32x2 *>(a.part_ml + 2 * at) = q35_f32x2{top, l};
-      } else {
-        *reinterpret_cast<q35_f32x4 *>(a.out + head * HD + dim) =
-            tree_finish(o, l, a.gates != nullptr ? a.gates + head * HD + dim : nullptr);
+        for (int i = 0; i < 4; ++i) {
+          x[i] = lo[i] * down;
+          x[4 + i] = hi[i] * down;
+        }
+        q35_split_f16(x, qhi[kk], qlo[kk]);
       }
     }
+    q35_f32x4 acc[NV];  // dims 16 n + 4 quad + i of the lane's vector
+#pragma unroll
+    for (int n = 0; n < NV; ++n) acc[n] = q35_f32x4{0.0F, 0.0F, 0.0F, 0.0F};
+    // the lane's vector: weights are 2^(score - ref); the sum is over its own tokens
+    float ref = -INFINITY, sum = 0.0F;
+
+    // 32 rows, K at cache[kb] and V a block behind it, the first of them the
+    // request's row t. (Rows past the request repeat one before them under a
+    // weight of 0; where such a row is not finite the request is marked.)
+    auto tile = [&](int kb, const int *at, int t) {
+      const uint32_t lost = static_cast<uint32_t>(q35_ballot(at[lane & 31] < 0));
+      q35_f32x4 s[2];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) s[k] = q35_f32x4{0.0F, 0.0F, 0.0F, 0.0F};
+      int krow[2];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) krow[k] = kb + (16 * k + col) * HD + 8 * (quad ^ ((16 * k + col) & (PIECES - 1)));
+#pragma unroll
+      for (int kk = 0; kk < KS; ++kk) {
+        q35_f16x8 x[2];  // piece 4 kk + quad of row r lies at that number xor r
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+          x[k] = q35_f16x8_bits(*reinterpret_cast<const q35_u32x4 *>(cache + (krow[k] ^ (32 * kk))));
+#pragma unroll
+        for (int k = 0; k < 2; ++k) s[k] = Q35_MFMA_F32_16X16X32_F16(x[k], qhi[kk], s[k]);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) s[k] = Q35_MFMA_F32_16X16X32_F16(x[k], qlo[kk], s[k]);
+      }
+      if (t + kTileTokens > rq.context || lost != 0u) {
+        const uint32_t seen = tree_visible(words, a.mask_words, t, rq.context, rq.len);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int tok = slot_token(i, quad);
+          float x = (lost >> tok) & 1u ? NAN : s[i >> 2][i & 3];  // a page outside the pool
+          s[i >> 2][i & 3] = (seen >> tok) & 1u ? x : -INFINITY;
+        }
+      }
+      float top = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) top = fmaxf(top, s[i >> 2][i & 3]);
+      top = q35_max_rows(top);
+      const float next = fmaxf(ref, score_ref(top, sscale)), least = next == -INFINITY ? 0.0F : next;
+      const float keep = ref == next ? 1.0F : Q35_EXP2(ref - least);  // 0 at the first seen row
+      float p[8], sums = 0.0F;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        p[i] = score_weight(s[i >> 2][i & 3], sscale, least);
+        sums += p[i];
+      }
+      sum = fmaf(sum, keep, sums);
+      ref = next;
+      if (q35_ballot(keep != 1.0F) != 0ull) {
+#pragma unroll
+        for (int n = 0; n < NV; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[n][i] *= keep;
+      }
+      q35_f16x8 phi, plo;
+      q35_split_f16(p, phi, plo);
+      // dims 16 n .. + 15 of row r: pair n of pieces, at that number xor r
+      const int r = 4 * quad + (col >> 2), vrow = kb + BLOCK + r * HD + 16 * (r & (PIECES / 2 - 1)) + 4 * (col & 3);
+#pragma unroll
+      for (int n = 0; n < NV; ++n) {
+        const uint16_t *v = cache + (vrow ^ (16 * n));
+        const q35_u32x2 lo = q35_lds_read_tr16(v), hi = q35_lds_read_tr16(v + 16 * HD);
+        const q35_f16x8 x = q35_f16x8_bits(q35_u32x4{lo[0], lo[1], hi[0], hi[1]});
+        acc[n] = Q35_MFMA_F32_16X16X32_F16(x, phi, acc[n]);
+        acc[n] = Q35_MFMA_F32_16X16X32_F16(x, plo, acc[n]);
+      }
+    };
+
+    // One barrier a stage: behind it the stage's loads of all wavefronts are in,
+    // and every wavefront is done with the stage before, whose place the next
+    // loads take. The pages of the rows after those are read a stage ahead, and
+    // looked at only behind the next wait.
+    for (int s = s0; s < s1; ++s) {
+      Q35_WAIT_VM(0);
+      if (tid < kStageTokens) sh.rows[(s + 2) & 3][tid] = stage_row(s + 2, following);
+      lds_barrier();
+      if (s + 1 < s1) issue(s + 1);
+      if (tid < kStageTokens) following = stage_page(s + 3);
+      if (active) {
+        const int t = kStageTokens * s;
+        for (int k = shared ? part : 0; k < (shared ? part + 1 : 2); ++k)
+          if (t + kTileTokens * k < rq.len)
+            tile((s & 1) * 2 * BLOCK + kTileTokens * k * HD, sh.rows[s & 3] + kTileTokens * k, t + kTileTokens * k);
+      }
+    }
+    lds_barrier();  // every wavefront is done with the last stage
+
+    // shared groups: the second wavefront's part through LDS, lane by lane
+    sum += __shfl_xor(sum, 16, 64);
+    sum += __shfl_xor(sum, 32, 64);
+    q35_f32x4 *join = reinterpret_cast<q35_f32x4 *>(cache) + static_cast<size_t>(shared ? group : 0) * (NV * 64);
+    if (shared && active && part == 1) {
+      sh.stat[group][0][lane] = ref;
+      sh.stat[group][1][lane] = sum;
+#pragma unroll
+      for (int n = 0; n < NV; ++n) join[n * 64 + lane] = acc[n];
+    }
+    if (shared) lds_barrier();
+    if (active && part == 0) {
+      if (shared) {
+        const float ref1 = sh.stat[group][0][lane], next = fmaxf(ref, ref1), least = next == -INFINITY ? 0.0F : next;
+        const float w0 = Q35_EXP2(ref - least), w1 = Q35_EXP2(ref1 - least);
+        ref = next;
+        sum = fmaf(sum, w0, sh.stat[group][1][lane] * w1);
+#pragma unroll
+        for (int n = 0; n < NV; ++n) {
+          const q35_f32x4 o = join[n * 64 + lane];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[n][i] = fmaf(o[i], w1, acc[n][i] * w0);
+        }
+      }
+      const bool whole = s0 == 0 && s1 == stages;
+      const size_t place = (2 * static_cast<size_t>(w) + (s0 == 0 ? 1 : 0)) * kBlockVectors + kGroupVectors * group + col;
+      if (live && !whole && quad == 0) {
+        a.part_ml[2 * place] = ref;
+        a.part_ml[2 * place + 1] = sum;
+      }
+#pragma unroll
+      for (int n = 0; n < NV; ++n) {
+        const int dim = 16 * n + 4 * quad;
+        const float y[4] = {acc[n][0], acc[n][1], acc[n][2], acc[n][3]};
+        if (!live) continue;
+        if (whole) tree_store<4>(a.out + head * HD + dim, y, sum, a.gates != nullptr ? a.gates + head * HD + dim : nullptr);
+        else tree_store<4>(a.part_o + place * HD + dim, y);
+      }
+    }
+    lds_barrier();  // the join and the row lists are free for the next item
   }
 }
 
-// The ranges' parts of one (node, head): weights exp(m_s - M), in range order.
+// Marked requests, one wavefront per (node, head): the formula row by row over
+// the rows that the node sees, each lane with its dims.
 template <int HD>
-__global__ __launch_bounds__(HD / 4) void tree_merge_kernel(TreeArgs a) {
-  const int h = static_cast<int>(blockIdx.x), i = static_cast<int>(blockIdx.y), b = static_cast<int>(blockIdx.z);
-  const TreeRequest rq = tree_request(a, b);
-  if (!rq.valid || i >= rq.nodes) return;
-  const int used = (rq.len + a.split_tokens - 1) / a.split_tokens, d = 4 * threadIdx.x;
-  const size_t head = static_cast<size_t>(rq.row0 + i) * a.heads + h, step = static_cast<size_t>(a.rows) * a.heads;
-  float top = -INFINITY;
-  for (int s = 0; s < used; ++s) top = fmaxf(top, a.part_ml[2 * (s * step + head)]);
-  const float base = top == -INFINITY ? 0.0F : top;
-  q35_f32x4 o = {0.0F, 0.0F, 0.0F, 0.0F};
-  float l = 0.0F;
-  for (int s = 0; s < used; ++s) {
-    const size_t at = s * step + head;
-    const float w = exp2f(a.part_ml[2 * at] - base);
-    l = fmaf(a.part_ml[2 * at + 1], w, l);
-    const q35_f32x4 x = *reinterpret_cast<const q35_f32x4 *>(a.part_o + at * HD + d);
+__device__ __forceinline__ void tree_row_by_row(const TreeArgs &a, const TreeRequest &rq, int i, int h, int b) {
+  constexpr int PER = HD / 64;
+  const int lane = threadIdx.x, g = h / (a.heads / a.kv_heads);
+  const size_t kvw = static_cast<size_t>(a.kv_heads) * HD, head = (static_cast<size_t>(rq.row0 + i) * a.heads + h) * HD + PER * lane;
+  const int32_t *table = a.page_table + static_cast<size_t>(b) * a.max_pages;
+  const uint64_t *words = a.masks + static_cast<size_t>(rq.row0 + i) * a.mask_words;
+  float x[PER], o[PER], mx = -INFINITY, l = 0.0F;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] = fmaf(x[e], w, o[e]);
+  for (int e = 0; e < PER; ++e) {
+    x[e] = a.q[head + e];
+    o[e] = 0.0F;
   }
-  *reinterpret_cast<q35_f32x4 *>(a.out + head * HD + d) =
-      tree_finish(o, l, a.gates != nullptr ? a.gates + head * HD + d : nullptr);
+  for (int t = 0; t < rq.len; ++t) {
+    const int j = t - rq.context;
+    if (j >= 0 && !((words[j >> 6] >> (j & 63)) & 1ull)) continue;
+    const int page = table[t >> a.page_shift];
+    const bool ok = static_cast<unsigned>(page) < static_cast<unsigned>(a.total_pages);
+    const size_t at = static_cast<size_t>(((ok ? page : 0) << a.page_shift) + (t & ((1 << a.page_shift) - 1))) * kvw +
+                      static_cast<size_t>(g) * HD + PER * lane;
+    float dot = 0.0F;
+#pragma unroll
+    for (int e = 0; e < PER; ++e) dot = fmaf(x[e], half_bits_to_float(a.k_pool[at + e]), dot);
+    const float s = ok ? group_sum<64>(dot) * (a.scale * 1.44269504088896341F) : NAN;
+    const float next = fmaxf(mx, s), least = next == -INFINITY ? 0.0F : next;
+    const float keep = mx == next ? 1.0F : exp2f(mx - least), p = exp2f(s - least);
+    mx = next;
+    l = fmaf(l, keep, p);
+#pragma unroll
+    for (int e = 0; e < PER; ++e) o[e] = fmaf(p, half_bits_to_float(a.v_pool[at + e]), o[e] * keep);
+  }
+  tree_store<PER>(a.out + head, o, l, a.gates != nullptr ? a.gates + head : nullptr);
+}
+
+// One wavefront per (node, head): the parts of its item, weights exp(m_w - M),
+// in workgroup order (the workgroups follow from the unit counts). Requests
+// that are refused on the device get NaN in their rows, where those are known.
+template <int HD>
+__global__ __launch_bounds__(64) void tree_merge_kernel(TreeArgs a) {
+  constexpr int PER = HD / 64;
+  const int i = static_cast<int>(blockIdx.x), h = static_cast<int>(blockIdx.y), b = static_cast<int>(blockIdx.z), lane = threadIdx.x;
+  const TreeRequest rq = tree_request(a, b);
+  if (!rq.valid) {
+    for (int r = i; r < rq.nodes; r += static_cast<int>(gridDim.x))
+#pragma unroll
+      for (int e = 0; e < PER; ++e)
+        a.out[(static_cast<size_t>(rq.row0 + r) * a.heads + h) * HD + PER * lane + e] = __uint_as_float(0x7fc00000u);
+    return;
+  }
+  if (i >= rq.nodes) return;
+  if (a.marks[b] != 0) {
+    tree_row_by_row<HD>(a, rq, i, h, b);
+    return;
+  }
+  const int qpk = a.heads / a.kv_heads, g = h / qpk, m = i * qpk + (h - g * qpk), stages = item_stages(rq);
+  const long long total = a.first_units[a.batch];
+  const long long first = a.first_units[b] + (static_cast<long long>(g) * item_blocks(a, rq) + m / kBlockVectors) * stages;
+  const int ranges = unit_groups(a, total);
+  const int w0 = unit_group(first, total, ranges), w1 = unit_group(first + stages - 1, total, ranges);
+  if (w0 == w1) return;  // finished by its workgroup
+  const size_t at = m % kBlockVectors;
+  auto place = [&](int w) { return (2 * static_cast<size_t>(w) + (w == w0 ? 1 : 0)) * kBlockVectors + at; };
+  float top = -INFINITY;
+  for (int w = w0; w <= w1; ++w) top = fmaxf(top, a.part_ml[2 * place(w)]);
+  const float least = top == -INFINITY ? 0.0F : top;
+  float o[PER], l = 0.0F;
+#pragma unroll
+  for (int e = 0; e < PER; ++e) o[e] = 0.0F;
+  for (int w = w0; w <= w1; ++w) {
+    const size_t p = place(w);
+    const float weight = exp2f(a.part_ml[2 * p] - least);
+    l = fmaf(a.part_ml[2 * p + 1], weight, l);
+#pragma unroll
+    for (int e = 0; e < PER; ++e) o[e] = fmaf(a.part_o[p * HD + PER * lane + e], weight, o[e]);
+  }
+  const size_t head = (static_cast<size_t>(rq.row0 + i) * a.heads + h) * HD + PER * lane;
+  tree_store<PER>(a.out + head, o, l, a.gates != nullptr ? a.gates + head : nullptr);
 }
 
 // ------------------------------------------------------------- acceptance
@@ -422,11 +589,10 @@ __global__ __launch_bounds__(64) void tree_accept_kernel(AcceptArgs a) {
 }  // namespace
 
 hipError_t launch_tree_attention(const TreeArgs &a, hipStream_t stream) {
-  const int blocks = (a.max_nodes * (a.heads / a.kv_heads) + kBlockVectors - 1) / kBlockVectors;
-  const dim3 grid(a.splits, blocks * a.kv_heads, a.batch), merge(a.heads, a.max_nodes, a.batch);
-#define Q35_TREE(HD)                                                                             \
-  Q35_LAUNCH((tree_attention_kernel<HD>), grid, dim3(64 * kTreeWaves), 0, stream, a);            \
-  if (a.splits > 1) Q35_LAUNCH((tree_merge_kernel<HD>), merge, dim3((HD) / 4), 0, stream, a);
+  const dim3 grid(a.groups + std::min(a.batch, 64)), merge(a.max_nodes, a.heads, a.batch);
+#define Q35_TREE(HD)                                                                  \
+  Q35_LAUNCH((tree_attention_kernel<HD>), grid, dim3(64 * kTreeWaves), 0, stream, a); \
+  Q35_LAUNCH((tree_merge_kernel<HD>), merge, dim3(64), 0, stream, a);
   switch (a.head_dim) {
     case 64: Q35_TREE(64) break;
     case 128: Q35_TREE(128) break;
@@ -437,17 +603,21 @@ hipError_t launch_tree_attention(const TreeArgs &a, hipStream_t stream) {
   return hipGetLastError();
 }
 
-// Ranges of cache rows per request: as many as give each CU two workgroups
-// (a workgroup's four wavefronts fill its SIMDs), each of whole rounds of the
-// four wavefronts' tiles.
-void tree_plan(int batch, int max_nodes, int max_len, int heads, int kv_heads, int cu_count, int *split_tokens, int *splits) {
-  constexpr int kRound = kTileTokens * kTreeWaves;
-  const long long blocks = static_cast<long long>((max_nodes * (heads / kv_heads) + kBlockVectors - 1) / kBlockVectors) * kv_heads * batch;
-  const int rounds = std::max(1, (max_len + kRound - 1) / kRound);
-  const int want = static_cast<int>(std::max(1LL, std::min<long long>(rounds, (2LL * cu_count + blocks - 1) / blocks)));
-  const int per = (rounds + want - 1) / want;
-  *split_tokens = per * kRound;
-  *splits = (rounds + per - 1) / per;
+// Workgroups of a launch: one per CU, but not more than the units that the
+// bounds allow.
+int tree_groups(int batch, int max_nodes, int max_len, int heads, int kv_heads, int cu_count) {
+  const long long blocks = (max_nodes * (heads / kv_heads) + kBlockVectors - 1) / kBlockVectors;
+  const long long units = blocks * kv_heads * batch * ((max_len + kStageTokens - 1) / kStageTokens);
+  return static_cast<int>(std::max(1LL, std::min<long long>(units, cu_count)));
+}
+
+size_t tree_workspace_bytes(const TreeArgs &a, size_t *marks, size_t *part_o, size_t *part_ml) {
+  auto align = [](size_t n) { return (n + 255) & ~static_cast<size_t>(255); };
+  const size_t parts = 2 * static_cast<size_t>(a.groups) * kBlockVectors;
+  *marks = align((static_cast<size_t>(a.batch) + 1) * 8);
+  *part_o = *marks + align(static_cast<size_t>(a.batch) * 4);
+  *part_ml = *part_o + align(parts * a.head_dim * 4);
+  return *part_ml + align(parts * 8);
 }
 
 hipError_t launch_tree_accept(const AcceptArgs &a, hipStream_t stream) {
