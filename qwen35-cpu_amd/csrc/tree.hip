@@ -18,6 +18,7 @@ constexpr int kTileTokens = 32;    // cache rows per tile
 constexpr int kStageTokens = 64;   // cache rows per stage: two tiles
 constexpr int kGroupVectors = 16;  // query vectors (node, head) per wavefront
 constexpr int kTreeWaves = 8;
+constexpr int kRowStages = kTreeWaves;  // stages whose rows are resolved at once, one per wavefront
 constexpr int kBlockVectors = kTreeWaves * kGroupVectors;  // query vectors per item
 // Probabilities are taken relative to the running maximum less 14 binades: as
 // two binary16 operands (22 bits) they then reach down to 2^-38 of the largest.
@@ -81,55 +82,84 @@ __device__ __forceinline__ uint32_t tree_visible(const uint64_t *words, int word
   return end - t < kTileTokens ? bits & ((1u << (end - t)) - 1u) : bits;
 }
 
-// N consecutive dims of an output (or of a part of one): normalised by the sum
-// l -- a zero sum saw nothing -- and gated.
-template <int N>
-__device__ __forceinline__ void tree_store(float *dst, const float y[N]) {
-#pragma unroll
-  for (int e = 0; e < N; e += 4) {
-    if constexpr (N >= 4) *reinterpret_cast<q35_f32x4 *>(dst + e) = q35_f32x4{y[e], y[e + 1], y[e + 2], y[e + 3]};
-    else if constexpr (N == 2) *reinterpret_cast<q35_f32x2 *>(dst) = q35_f32x2{y[0], y[1]};
-    else dst[0] = y[0];
-  }
-}
-template <int N>
-__device__ __forceinline__ void tree_store(float *dst, const float y[N], float l, const float *gates) {
+// Four dims of an output: normalised by the sum l -- a zero sum saw nothing --
+// and gated.
+__device__ __forceinline__ void tree_store(float *dst, q35_f32x4 y, float l, const float *gates) {
   const float inv = 1.0F / (l == 0.0F ? 1.0F : l);
-  float z[N];
+  q35_f32x4 gate = {0.0F, 0.0F, 0.0F, 0.0F};
+  if (gates != nullptr) gate = *reinterpret_cast<const q35_f32x4 *>(gates);
 #pragma unroll
-  for (int e = 0; e < N; ++e) z[e] = y[e] * inv;
-  if (gates != nullptr) {
-#pragma unroll
-    for (int e = 0; e < N; ++e) z[e] *= sigmoid_stable(gates[e]);
+  for (int e = 0; e < 4; ++e) {
+    y[e] *= inv;
+    if (gates != nullptr) y[e] *= sigmoid_stable(gate[e]);
   }
-  tree_store<N>(dst, z);
+  *reinterpret_cast<q35_f32x4 *>(dst) = y;
 }
 
-// The work is cut into units of one stage (64 cache rows) of one item (request,
-// KV head, block of up to 128 query vectors), items one after the other and the
-// stages of an item in order; request b has tree_units(b) of them. Workgroup w
-// of W takes units [w T / W, (w + 1) T / W) of all T, so ragged contexts leave
-// every CU the same share, whatever the host knew of the lengths. An item that
-// lies inside one workgroup's range is finished there; of the others each
-// workgroup leaves a part (maximum, sum, unnormalised output) in one of its two
-// places: the second where its range holds the item's first unit, else the
-// first (a range has at most one of each).
+// The work is cut into items (request, KV head, block of up to 128 query
+// vectors), items one after the other, and an item into units: kItemUnits for
+// its beginning and end (queries, first loads and results take about as long as
+// three stages) and one per stage of 64 cache rows. Workgroup w of W takes units
+// [w T / W, (w + 1) T / W) of all T, so ragged contexts leave every CU the same
+// share, whatever the host knew of the lengths. An item whose stages lie inside
+// one workgroup's range is finished there; of the others each workgroup with
+// some of the stages leaves a part (maximum, sum, unnormalised output) in one of
+// its two places: the second where it has the item's first stage, else the first
+// (a range has at most one of each).
+constexpr int kItemUnits = 3;
 __device__ __forceinline__ int item_blocks(const TreeArgs &a, const TreeRequest &r) {
   return (r.nodes * (a.heads / a.kv_heads) + kBlockVectors - 1) / kBlockVectors;
 }
 __device__ __forceinline__ int item_stages(const TreeRequest &r) { return (r.len + kStageTokens - 1) / kStageTokens; }
 __device__ __forceinline__ long long tree_units(const TreeArgs &a, int b) {
   const TreeRequest r = tree_request(a, b);
-  return static_cast<long long>(a.kv_heads) * item_blocks(a, r) * item_stages(r);
+  return static_cast<long long>(a.kv_heads) * item_blocks(a, r) * (r.nodes > 0 ? item_stages(r) + kItemUnits : 0);
 }
 // W: the launched workgroups, or as many as there are units, so that no range
 // before the last is empty.
 __device__ __forceinline__ int unit_groups(const TreeArgs &a, long long total) {
   return total < a.groups ? static_cast<int>(max(total, 1LL)) : a.groups;
 }
-__device__ __forceinline__ long long unit_begin(long long w, long long total, int groups) { return w * total / groups; }
+// (Quotients of whole numbers below 2^44 by whole numbers below 2^31 or 2^9: in
+// fp64 they round to no wrong floor, and take a tenth of the integer code.)
+__device__ __forceinline__ long long unit_begin(int w, long long total, int groups) {
+  return static_cast<long long>(floor(static_cast<double>(w * total) / groups));
+}
 __device__ __forceinline__ int unit_group(long long unit, long long total, int groups) {
-  return static_cast<int>(((unit + 1) * groups - 1) / total);
+  return static_cast<int>(floor(static_cast<double>((unit + 1) * groups - 1) / static_cast<double>(total)));
+}
+
+// The formula row by row over the rows that a node sees, one wavefront for one
+// (node, head): for items with values that are not finite among their nodes.
+template <int HD>
+__device__ void tree_row_by_row(const TreeArgs &a, const TreeRequest &rq, int i, int h, int b) {
+  constexpr int F = HD / 4;  // lanes past the dims repeat them
+  const int f = threadIdx.x & (F - 1), g = h / (a.heads / a.kv_heads);
+  const size_t kvw = static_cast<size_t>(a.kv_heads) * HD, head = (static_cast<size_t>(rq.row0 + i) * a.heads + h) * HD + 4 * f;
+  const int32_t *table = a.page_table + static_cast<size_t>(b) * a.max_pages;
+  const uint64_t *words = a.masks + static_cast<size_t>(rq.row0 + i) * a.mask_words;
+  const q35_f32x4 x = *reinterpret_cast<const q35_f32x4 *>(a.q + head);
+  q35_f32x4 o = {0.0F, 0.0F, 0.0F, 0.0F};
+  float mx = -INFINITY, l = 0.0F;
+  for (int t = 0; t < rq.len; ++t) {
+    const int j = t - rq.context;
+    if (j >= 0 && !((words[j >> 6] >> (j & 63)) & 1ull)) continue;
+    const int page = table[t >> a.page_shift];
+    const bool ok = static_cast<unsigned>(page) < static_cast<unsigned>(a.total_pages);
+    const size_t at = static_cast<size_t>(((ok ? page : 0) << a.page_shift) + (t & ((1 << a.page_shift) - 1))) * kvw +
+                      static_cast<size_t>(g) * HD + 4 * f;
+    float dot = 0.0F;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) dot = fmaf(x[e], half_bits_to_float(a.k_pool[at + e]), dot);
+    const float s = ok ? group_sum<F>(dot) * (a.scale * 1.44269504088896341F) : NAN;
+    const float next = fmaxf(mx, s), least = next == -INFINITY ? 0.0F : next;
+    const float keep = mx == next ? 1.0F : Q35_EXP2(mx - least), p = Q35_EXP2(s - least);
+    mx = next;
+    l = fmaf(l, keep, p);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = fmaf(p, half_bits_to_float(a.v_pool[at + e]), o[e] * keep);
+  }
+  tree_store(a.out + head, o, l, a.gates != nullptr ? a.gates + head : nullptr);
 }
 
 // One workgroup of eight wavefronts. A stage's K and V rows go straight from
@@ -159,11 +189,11 @@ __global__ __launch_bounds__(64 * kTreeWaves) Q35_WAVES_PER_EU(2) void tree_atte
   // are needed are the ones at the barriers.)
   __shared__ struct __align__(1024) {
     uint16_t cache[4 * BLOCK];       // [stage % 2][K, V][row][dim]
-    int rows[4][kStageTokens];       // cache rows of four stages (-1: none)
-    float stat[4][2][64];
-    long long scan[64 * kTreeWaves];
+    int rows[2 * kRowStages][kStageTokens];  // cache rows of two runs of stages (-1: none)
+    float stat[kTreeWaves][2][kGroupVectors];
+    long long units[kTreeWaves];
     long long first_unit;
-    int first_request, marked;
+    int first_request, special;
   } sh;
   uint16_t *cache = sh.cache;
   const int tid = threadIdx.x, wave = q35_uniform(tid >> 6), lane = tid & 63, col = lane & 15, quad = lane >> 4;
@@ -171,51 +201,27 @@ __global__ __launch_bounds__(64 * kTreeWaves) Q35_WAVES_PER_EU(2) void tree_atte
   const size_t kvw = static_cast<size_t>(a.kv_heads) * HD;
   const int shift = a.page_shift, pmask = (1 << shift) - 1;
 
-  // The workgroups behind those of the units mark each request with an infinite
-  // or NaN value in a node's row: products with probabilities of 0 would carry
-  // it to nodes that do not see the row, so the merge computes such requests
-  // anew.
-  if (w >= a.groups) {
-    for (int b = w - a.groups; b < a.batch; b += static_cast<int>(gridDim.x) - a.groups) {
-      const TreeRequest rq = tree_request(a, b);
-      if (tid == 0) sh.marked = 0;
-      __syncthreads();
-      const int32_t *table = a.page_table + static_cast<size_t>(b) * a.max_pages;
-      const int pieces = static_cast<int>(kvw / 8);
-      bool special = false;
-      for (int e = tid; rq.valid && e < rq.nodes * pieces; e += 64 * kTreeWaves) {
-        const int t = rq.context + e / pieces, page = table[t >> shift];
-        if (static_cast<unsigned>(page) >= static_cast<unsigned>(a.total_pages)) continue;
-        const q35_u32x4 v = *reinterpret_cast<const q35_u32x4 *>(
-            a.v_pool + static_cast<size_t>((page << shift) + (t & pmask)) * kvw + 8 * static_cast<size_t>(e % pieces));
-#pragma unroll
-        for (int d = 0; d < 4; ++d) special |= (v[d] & 0x7c00u) == 0x7c00u || (v[d] & 0x7c000000u) == 0x7c000000u;
-      }
-      if (special) sh.marked = 1;
-      __syncthreads();
-      if (tid == 0) a.marks[b] = sh.marked;
-      __syncthreads();
-    }
-    return;
-  }
-
   // running unit counts over the requests, a run of them per thread
   const int run = (a.batch + 64 * kTreeWaves - 1) / (64 * kTreeWaves), b0 = min(tid * run, a.batch), b1 = min(b0 + run, a.batch);
   long long mine = 0;
   for (int b = b0; b < b1; ++b) mine += tree_units(a, b);
-  sh.scan[tid] = mine;
-  __syncthreads();
-  for (int d = 1; d < 64 * kTreeWaves; d <<= 1) {
-    const long long up = tid >= d ? sh.scan[tid - d] : 0;
-    __syncthreads();
-    sh.scan[tid] += up;
-    __syncthreads();
+  long long through = mine;  // inclusive, over the wavefront and then over all
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const long long up = __shfl(through, max(lane - d, 0), 64);
+    if (lane >= d) through += up;
   }
-  const long long total = sh.scan[64 * kTreeWaves - 1];
+  if (lane == 63) sh.units[wave] = through;
+  __syncthreads();
+  long long total = 0;
+  for (int v = 0; v < kTreeWaves; ++v) {
+    if (v < wave) through += sh.units[v];
+    total += sh.units[v];
+  }
   const int ranges = unit_groups(a, total);
   const long long begin = unit_begin(min(w, ranges), total, ranges), end = unit_begin(min(w + 1, ranges), total, ranges);
   {
-    long long at = sh.scan[tid] - mine;
+    long long at = through - mine;
     for (int b = b0; b < b1; ++b) {
       const long long n = tree_units(a, b);
       if (w == 0) a.first_units[b] = at;  // for the merge
@@ -235,16 +241,19 @@ __global__ __launch_bounds__(64 * kTreeWaves) Q35_WAVES_PER_EU(2) void tree_atte
   for (long long unit = begin; unit < end;) {
     const TreeRequest rq = tree_request(a, b);
     const int stages = item_stages(rq), blocks = item_blocks(a, rq);
-    const long long request_units = static_cast<long long>(a.kv_heads) * blocks * stages;
+    const int item_units = stages + kItemUnits;
+    const long long request_units = rq.nodes > 0 ? static_cast<long long>(a.kv_heads) * blocks * item_units : 0;
     if (unit >= base + request_units) {  // (a request without units among them)
       base += request_units;
       ++b;
       continue;
     }
-    const int item = static_cast<int>((unit - base) / stages), s0 = static_cast<int>((unit - base) - static_cast<long long>(item) * stages);
-    const int s1 = static_cast<int>(min(static_cast<long long>(stages), s0 + (end - unit)));
+    const int item = static_cast<int>(unit - base) / item_units, u0 = static_cast<int>(unit - base) - item * item_units;
+    const int u1 = static_cast<int>(min(static_cast<long long>(item_units), u0 + (end - unit)));
+    const int s0 = max(0, u0 - kItemUnits), s1 = u1 - kItemUnits;
+    unit += u1 - u0;
+    if (s1 <= s0) continue;  // only the item's beginning: the next workgroup has its first stage
     const int g = item / blocks, m0 = (item - g * blocks) * kBlockVectors;
-    unit += s1 - s0;
 
     const int vectors = rq.nodes * qpk, groups = min(kTreeWaves, (vectors - m0 + kGroupVectors - 1) / kGroupVectors);
     const bool shared = groups <= kTreeWaves / 2;  // two wavefronts to a group of vectors
@@ -253,18 +262,21 @@ __global__ __launch_bounds__(64 * kTreeWaves) Q35_WAVES_PER_EU(2) void tree_atte
     const int mg = m0 + kGroupVectors * group;
 
     const int32_t *table = a.page_table + static_cast<size_t>(b) * a.max_pages;
-    // token `tid` of stage s (tokens past the request: the stage's first), its
-    // page, and from that its cache row
-    auto stage_token = [&](int s) {
-      const int t = kStageTokens * min(s, s1 - 1);
-      return t + tid < rq.len ? t + tid : t;
+    // The cache rows of the stages, a run of kRowStages at a time (a token per
+    // thread): token `tid` of run c (past the request: its stage's first), its
+    // page, and from that its row.
+    auto run_token = [&](int c) {
+      const int t = kStageTokens * min(s0 + kRowStages * c + wave, s1 - 1);
+      return t + lane < rq.len ? t + lane : t;
     };
-    auto stage_page = [&](int s) { return table[stage_token(s) >> shift]; };
-    auto stage_row = [&](int s, int page) {
-      return static_cast<unsigned>(page) < static_cast<unsigned>(a.total_pages) ? (page << shift) + (stage_token(s) & pmask) : -1;
+    auto run_page = [&](int c) { return table[run_token(c) >> shift]; };
+    auto keep_rows = [&](int c, int page) {
+      sh.rows[kRowStages * (c & 1) + wave][lane] =
+          static_cast<unsigned>(page) < static_cast<unsigned>(a.total_pages) ? (page << shift) + (run_token(c) & pmask) : -1;
     };
+    auto stage_rows = [&](int s) { return sh.rows[(s - s0) & (2 * kRowStages - 1)]; };
     auto issue = [&](int s) {
-      const int *at = sh.rows[s & 3];
+      const int *at = stage_rows(s);
       const uint16_t *kp = a.k_pool + static_cast<size_t>(g) * HD, *vp = a.v_pool + static_cast<size_t>(g) * HD;
 #pragma unroll
       for (int i = 0; i < LOADS; ++i) {
@@ -275,17 +287,13 @@ __global__ __launch_bounds__(64 * kTreeWaves) Q35_WAVES_PER_EU(2) void tree_atte
         Q35_LOAD_LDS16(vp + row + 8 * (slot ^ (2 * r & (PIECES - 1))), to + BLOCK);
       }
     };
-    if (tid < kStageTokens) {
-      const int page0 = stage_page(s0), page1 = stage_page(s0 + 1);
-      sh.rows[s0 & 3][tid] = stage_row(s0, page0);
-      sh.rows[(s0 + 1) & 3][tid] = stage_row(s0 + 1, page1);
-    }
-    int following = tid < kStageTokens ? stage_page(s0 + 2) : 0;
+    if (tid == 0) sh.special = 0;
+    keep_rows(0, run_page(0));
+    int following = run_page(1);
     lds_barrier();
     issue(s0);
 
     // the lane's query vector (spare lanes repeat the last one and store nothing)
-    const bool live = mg + col < vectors;
     const int m = min(mg + col, vectors - 1), node = m / qpk, u = m - node * qpk;
     const size_t head = static_cast<size_t>(rq.row0 + node) * a.heads + g * qpk + u;
     const uint64_t *words = a.masks + static_cast<size_t>(rq.row0 + node) * a.mask_words;
@@ -334,7 +342,7 @@ __global__ __launch_bounds__(64 * kTreeWaves) Q35_WAVES_PER_EU(2) void tree_atte
 
     // 32 rows, K at cache[kb] and V a block behind it, the first of them the
     // request's row t. (Rows past the request repeat one before them under a
-    // weight of 0; where such a row is not finite the request is marked.)
+    // weight of 0.)
     auto tile = [&](int kb, const int *at, int t) {
       const uint32_t lost = static_cast<uint32_t>(q35_ballot(at[lane & 31] < 0));
       q35_f32x4 s[2];
@@ -399,100 +407,101 @@ __global__ __launch_bounds__(64 * kTreeWaves) Q35_WAVES_PER_EU(2) void tree_atte
 
     // One barrier a stage: behind it the stage's loads of all wavefronts are in,
     // and every wavefront is done with the stage before, whose place the next
-    // loads take. The pages of the rows after those are read a stage ahead, and
-    // looked at only behind the next wait.
+    // loads take. A run's pages are read most of a run before they are looked at.
     for (int s = s0; s < s1; ++s) {
+      const int in_run = (s - s0) & (kRowStages - 1), c = (s - s0) / kRowStages;
       Q35_WAIT_VM(0);
-      if (tid < kStageTokens) sh.rows[(s + 2) & 3][tid] = stage_row(s + 2, following);
+      if (in_run == 1) keep_rows(c + 1, following);
       lds_barrier();
       if (s + 1 < s1) issue(s + 1);
-      if (tid < kStageTokens) following = stage_page(s + 3);
+      if (in_run == 2) following = run_page(c + 2);
+      const int t = kStageTokens * s;
+      if (t + kStageTokens > rq.context) {
+        // An infinite or NaN value in a node's row: products with weights of 0
+        // would carry it to nodes that do not see the row, so such an item is
+        // computed anew, row by row.
+        bool special = false;
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+          const int e = i * 64 * kTreeWaves + tid, r = t + e / PIECES;
+          const q35_u32x4 v = *reinterpret_cast<const q35_u32x4 *>(cache + (s & 1) * 2 * BLOCK + BLOCK + 8 * e);
+#pragma unroll
+          for (int d = 0; d < 4; ++d)
+            special |= r >= rq.context && r < rq.len && ((v[d] & 0x7c00u) == 0x7c00u || (v[d] & 0x7c000000u) == 0x7c000000u);
+        }
+        if (special) sh.special = 1;
+      }
       if (active) {
-        const int t = kStageTokens * s;
         for (int k = shared ? part : 0; k < (shared ? part + 1 : 2); ++k)
           if (t + kTileTokens * k < rq.len)
-            tile((s & 1) * 2 * BLOCK + kTileTokens * k * HD, sh.rows[s & 3] + kTileTokens * k, t + kTileTokens * k);
+            tile((s & 1) * 2 * BLOCK + kTileTokens * k * HD, stage_rows(s) + kTileTokens * k, t + kTileTokens * k);
       }
     }
     lds_barrier();  // every wavefront is done with the last stage
 
-    // shared groups: the second wavefront's part through LDS, lane by lane
+    // Each group's vectors through LDS, [vector][dims] with the 16-byte pieces
+    // of a row at their number xor the vector: first, of a shared group, the
+    // second wavefront's part, then the group's result, whose rows then leave
+    // whole, dealt over the wavefronts.
     sum += __shfl_xor(sum, 16, 64);
     sum += __shfl_xor(sum, 32, 64);
-    q35_f32x4 *join = reinterpret_cast<q35_f32x4 *>(cache) + static_cast<size_t>(shared ? group : 0) * (NV * 64);
+    constexpr int F = HD / 4;
+    q35_f32x4 *result = reinterpret_cast<q35_f32x4 *>(cache) + static_cast<size_t>(group) * (kGroupVectors * F) + col * F;
     if (shared && active && part == 1) {
-      sh.stat[group][0][lane] = ref;
-      sh.stat[group][1][lane] = sum;
+      sh.stat[wave][0][col] = ref;
+      sh.stat[wave][1][col] = sum;
 #pragma unroll
-      for (int n = 0; n < NV; ++n) join[n * 64 + lane] = acc[n];
+      for (int n = 0; n < NV; ++n) result[(4 * n + quad) ^ col] = acc[n];
     }
     if (shared) lds_barrier();
+    const bool whole = s0 == 0 && s1 == stages;
+    const size_t place = (2 * static_cast<size_t>(w) + (s0 == 0 ? 1 : 0)) * kBlockVectors;
     if (active && part == 0) {
       if (shared) {
-        const float ref1 = sh.stat[group][0][lane], next = fmaxf(ref, ref1), least = next == -INFINITY ? 0.0F : next;
+        const float *other = &sh.stat[wave + kTreeWaves / 2][0][0];
+        const float ref1 = other[col], next = fmaxf(ref, ref1), least = next == -INFINITY ? 0.0F : next;
         const float w0 = Q35_EXP2(ref - least), w1 = Q35_EXP2(ref1 - least);
         ref = next;
-        sum = fmaf(sum, w0, sh.stat[group][1][lane] * w1);
+        sum = fmaf(sum, w0, other[kGroupVectors + col] * w1);
 #pragma unroll
         for (int n = 0; n < NV; ++n) {
-          const q35_f32x4 o = join[n * 64 + lane];
+          const q35_f32x4 o = result[(4 * n + quad) ^ col];
 #pragma unroll
           for (int i = 0; i < 4; ++i) acc[n][i] = fmaf(o[i], w1, acc[n][i] * w0);
         }
       }
-      const bool whole = s0 == 0 && s1 == stages;
-      const size_t place = (2 * static_cast<size_t>(w) + (s0 == 0 ? 1 : 0)) * kBlockVectors + kGroupVectors * group + col;
-      if (live && !whole && quad == 0) {
-        a.part_ml[2 * place] = ref;
-        a.part_ml[2 * place + 1] = sum;
-      }
 #pragma unroll
-      for (int n = 0; n < NV; ++n) {
-        const int dim = 16 * n + 4 * quad;
-        const float y[4] = {acc[n][0], acc[n][1], acc[n][2], acc[n][3]};
-        if (!live) continue;
-        if (whole) tree_store<4>(a.out + head * HD + dim, y, sum, a.gates != nullptr ? a.gates + head * HD + dim : nullptr);
-        else tree_store<4>(a.part_o + place * HD + dim, y);
+      for (int n = 0; n < NV; ++n) result[(4 * n + quad) ^ col] = acc[n];
+      sh.stat[group][1][col] = sum;
+      if (!whole && quad == 0) {
+        a.part_ml[2 * (place + kGroupVectors * group + col)] = ref;
+        a.part_ml[2 * (place + kGroupVectors * group + col) + 1] = sum;
       }
     }
-    lds_barrier();  // the join and the row lists are free for the next item
+    lds_barrier();
+    const int count = min(kBlockVectors, vectors - m0);
+    if (sh.special != 0 && whole) {
+      for (int v = wave; v < count; v += kTreeWaves) {
+        const int vn = (m0 + v) / qpk;
+        tree_row_by_row<HD>(a, rq, vn, g * qpk + m0 + v - vn * qpk, b);
+      }
+    } else {
+      const int f = lane & (F - 1);
+#pragma unroll 4
+      for (int v = wave * (64 / F) + lane / F; v < count; v += kTreeWaves * (64 / F)) {
+        const q35_f32x4 y = reinterpret_cast<q35_f32x4 *>(cache)[v * F + (f ^ (v & (kGroupVectors - 1)))];
+        if (whole) {
+          const int vn = (m0 + v) / qpk, vu = m0 + v - vn * qpk;
+          const size_t to = (static_cast<size_t>(rq.row0 + vn) * a.heads + g * qpk + vu) * HD + 4 * f;
+          tree_store(a.out + to, y, sh.stat[v / kGroupVectors][1][v & (kGroupVectors - 1)], a.gates != nullptr ? a.gates + to : nullptr);
+        } else {
+          *reinterpret_cast<q35_f32x4 *>(a.part_o + (place + v) * HD + 4 * f) = y;
+        }
+      }
+    }
+    if (!whole && tid == 0) a.specials[2 * w + (s0 == 0 ? 1 : 0)] = sh.special;
+    lds_barrier();  // the results and the row lists are free for the next item
   }
-}
-
-// Marked requests, one wavefront per (node, head): the formula row by row over
-// the rows that the node sees, each lane with its dims.
-template <int HD>
-__device__ __forceinline__ void tree_row_by_row(const TreeArgs &a, const TreeRequest &rq, int i, int h, int b) {
-  constexpr int PER = HD / 64;
-  const int lane = threadIdx.x, g = h / (a.heads / a.kv_heads);
-  const size_t kvw = static_cast<size_t>(a.kv_heads) * HD, head = (static_cast<size_t>(rq.row0 + i) * a.heads + h) * HD + PER * lane;
-  const int32_t *table = a.page_table + static_cast<size_t>(b) * a.max_pages;
-  const uint64_t *words = a.masks + static_cast<size_t>(rq.row0 + i) * a.mask_words;
-  float x[PER], o[PER], mx = -INFINITY, l = 0.0F;
-#pragma unroll
-  for (int e = 0; e < PER; ++e) {
-    x[e] = a.q[head + e];
-    o[e] = 0.0F;
-  }
-  for (int t = 0; t < rq.len; ++t) {
-    const int j = t - rq.context;
-    if (j >= 0 && !((words[j >> 6] >> (j & 63)) & 1ull)) continue;
-    const int page = table[t >> a.page_shift];
-    const bool ok = static_cast<unsigned>(page) < static_cast<unsigned>(a.total_pages);
-    const size_t at = static_cast<size_t>(((ok ? page : 0) << a.page_shift) + (t & ((1 << a.page_shift) - 1))) * kvw +
-                      static_cast<size_t>(g) * HD + PER * lane;
-    float dot = 0.0F;
-#pragma unroll
-    for (int e = 0; e < PER; ++e) dot = fmaf(x[e], half_bits_to_float(a.k_pool[at + e]), dot);
-    const float s = ok ? group_sum<64>(dot) * (a.scale * 1.44269504088896341F) : NAN;
-    const float next = fmaxf(mx, s), least = next == -INFINITY ? 0.0F : next;
-    const float keep = mx == next ? 1.0F : exp2f(mx - least), p = exp2f(s - least);
-    mx = next;
-    l = fmaf(l, keep, p);
-#pragma unroll
-    for (int e = 0; e < PER; ++e) o[e] = fmaf(p, half_bits_to_float(a.v_pool[at + e]), o[e] * keep);
-  }
-  tree_store<PER>(a.out + head, o, l, a.gates != nullptr ? a.gates + head : nullptr);
 }
 
 // One wavefront per (node, head): the parts of its item, weights exp(m_w - M),
@@ -500,44 +509,67 @@ __device__ __forceinline__ void tree_row_by_row(const TreeArgs &a, const TreeReq
 // that are refused on the device get NaN in their rows, where those are known.
 template <int HD>
 __global__ __launch_bounds__(64) void tree_merge_kernel(TreeArgs a) {
-  constexpr int PER = HD / 64;
-  const int i = static_cast<int>(blockIdx.x), h = static_cast<int>(blockIdx.y), b = static_cast<int>(blockIdx.z), lane = threadIdx.x;
+  constexpr int F = HD / 4;  // lanes past the dims repeat them
+  const int i = static_cast<int>(blockIdx.x), h = static_cast<int>(blockIdx.y), b = static_cast<int>(blockIdx.z);
+  const int lane = threadIdx.x, f = lane & (F - 1);
   const TreeRequest rq = tree_request(a, b);
+  const long long total = a.first_units[a.batch], base = a.first_units[b];
   if (!rq.valid) {
     for (int r = i; r < rq.nodes; r += static_cast<int>(gridDim.x))
 #pragma unroll
-      for (int e = 0; e < PER; ++e)
-        a.out[(static_cast<size_t>(rq.row0 + r) * a.heads + h) * HD + PER * lane + e] = __uint_as_float(0x7fc00000u);
+      for (int e = 0; e < 4; ++e)
+        a.out[(static_cast<size_t>(rq.row0 + r) * a.heads + h) * HD + 4 * f + e] = __uint_as_float(0x7fc00000u);
     return;
   }
   if (i >= rq.nodes) return;
-  if (a.marks[b] != 0) {
-    tree_row_by_row<HD>(a, rq, i, h, b);
-    return;
-  }
   const int qpk = a.heads / a.kv_heads, g = h / qpk, m = i * qpk + (h - g * qpk), stages = item_stages(rq);
-  const long long total = a.first_units[a.batch];
-  const long long first = a.first_units[b] + (static_cast<long long>(g) * item_blocks(a, rq) + m / kBlockVectors) * stages;
+  const long long first =
+      base + (static_cast<long long>(g) * item_blocks(a, rq) + m / kBlockVectors) * (stages + kItemUnits) + kItemUnits;
   const int ranges = unit_groups(a, total);
   const int w0 = unit_group(first, total, ranges), w1 = unit_group(first + stages - 1, total, ranges);
   if (w0 == w1) return;  // finished by its workgroup
   const size_t at = m % kBlockVectors;
   auto place = [&](int w) { return (2 * static_cast<size_t>(w) + (w == w0 ? 1 : 0)) * kBlockVectors + at; };
+  // 64 parts at a time: a part's maximum and sum per lane
   float top = -INFINITY;
-  for (int w = w0; w <= w1; ++w) top = fmaxf(top, a.part_ml[2 * place(w)]);
-  const float least = top == -INFINITY ? 0.0F : top;
-  float o[PER], l = 0.0F;
-#pragma unroll
-  for (int e = 0; e < PER; ++e) o[e] = 0.0F;
-  for (int w = w0; w <= w1; ++w) {
-    const size_t p = place(w);
-    const float weight = exp2f(a.part_ml[2 * p] - least);
-    l = fmaf(a.part_ml[2 * p + 1], weight, l);
-#pragma unroll
-    for (int e = 0; e < PER; ++e) o[e] = fmaf(a.part_o[p * HD + PER * lane + e], weight, o[e]);
+  bool special = false;
+  for (int w = w0 + lane; w <= w1; w += 64) {
+    top = fmaxf(top, a.part_ml[2 * place(w)]);
+    special |= a.specials[2 * w + (w == w0 ? 1 : 0)] != 0;
   }
-  const size_t head = (static_cast<size_t>(rq.row0 + i) * a.heads + h) * HD + PER * lane;
-  tree_store<PER>(a.out + head, o, l, a.gates != nullptr ? a.gates + head : nullptr);
+  top = group_max<64>(top);
+  if (q35_ballot(special) != 0ull) {
+    tree_row_by_row<HD>(a, rq, i, h, b);
+    return;
+  }
+  const float least = top == -INFINITY ? 0.0F : top;
+  q35_f32x4 o = {0.0F, 0.0F, 0.0F, 0.0F};
+  float l = 0.0F;
+  for (int c = w0; c <= w1; c += 64) {
+    const int n = min(64, w1 - c + 1);
+    float weight = 0.0F, lw = 0.0F;
+    if (lane < n) {
+      const q35_f32x2 ml = *reinterpret_cast<const q35_f32x2 *>(a.part_ml + 2 * place(c + lane));
+      weight = Q35_EXP2(ml[0] - least);
+      lw = ml[1] * weight;
+    }
+    l += group_sum<64>(lw);
+    constexpr int U = 8;  // parts in flight
+    for (int k = 0; k < n; k += U) {
+      q35_f32x4 x[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) x[u] = *reinterpret_cast<const q35_f32x4 *>(a.part_o + place(c + min(k + u, n - 1)) * HD + 4 * f);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (k + u >= n) break;
+        const float w = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(weight), k + u));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = fmaf(x[u][e], w, o[e]);
+      }
+    }
+  }
+  const size_t head = (static_cast<size_t>(rq.row0 + i) * a.heads + h) * HD + 4 * f;
+  tree_store(a.out + head, o, l, a.gates != nullptr ? a.gates + head : nullptr);
 }
 
 // ------------------------------------------------------------- acceptance
@@ -589,7 +621,7 @@ __global__ __launch_bounds__(64) void tree_accept_kernel(AcceptArgs a) {
 }  // namespace
 
 hipError_t launch_tree_attention(const TreeArgs &a, hipStream_t stream) {
-  const dim3 grid(a.groups + std::min(a.batch, 64)), merge(a.max_nodes, a.heads, a.batch);
+  const dim3 grid(a.groups), merge(a.max_nodes, a.heads, a.batch);
 #define Q35_TREE(HD)                                                                  \
   Q35_LAUNCH((tree_attention_kernel<HD>), grid, dim3(64 * kTreeWaves), 0, stream, a); \
   Q35_LAUNCH((tree_merge_kernel<HD>), merge, dim3(64), 0, stream, a);
@@ -606,16 +638,18 @@ hipError_t launch_tree_attention(const TreeArgs &a, hipStream_t stream) {
 // Workgroups of a launch: one per CU, but not more than the units that the
 // bounds allow.
 int tree_groups(int batch, int max_nodes, int max_len, int heads, int kv_heads, int cu_count) {
-  const long long blocks = (max_nodes * (heads / kv_heads) + kBlockVectors - 1) / kBlockVectors;
-  const long long units = blocks * kv_heads * batch * ((max_len + kStageTokens - 1) / kStageTokens);
-  return static_cast<int>(std::max(1LL, std::min<long long>(units, cu_count)));
+  return static_cast<int>(std::max(1LL, std::min<long long>(tree_request_units(max_nodes, max_len, heads, kv_heads) * batch, cu_count)));
+}
+long long tree_request_units(int max_nodes, int max_len, int heads, int kv_heads) {
+  const long long blocks = (static_cast<long long>(max_nodes) * (heads / kv_heads) + kBlockVectors - 1) / kBlockVectors;
+  return blocks * kv_heads * ((static_cast<long long>(max_len) + kStageTokens - 1) / kStageTokens + kItemUnits);
 }
 
-size_t tree_workspace_bytes(const TreeArgs &a, size_t *marks, size_t *part_o, size_t *part_ml) {
+size_t tree_workspace_bytes(const TreeArgs &a, size_t *specials, size_t *part_o, size_t *part_ml) {
   auto align = [](size_t n) { return (n + 255) & ~static_cast<size_t>(255); };
   const size_t parts = 2 * static_cast<size_t>(a.groups) * kBlockVectors;
-  *marks = align((static_cast<size_t>(a.batch) + 1) * 8);
-  *part_o = *marks + align(static_cast<size_t>(a.batch) * 4);
+  *specials = align((static_cast<size_t>(a.batch) + 1) * 8);
+  *part_o = *specials + align(2 * static_cast<size_t>(a.groups) * 4);
   *part_ml = *part_o + align(parts * a.head_dim * 4);
   return *part_ml + align(parts * 8);
 }
