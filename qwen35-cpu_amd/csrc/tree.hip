@@ -99,14 +99,14 @@ __device__ __forceinline__ void tree_store(float *dst, q35_f32x4 y, float l, con
 // The work is cut into items (request, KV head, block of up to 128 query
 // vectors), items one after the other, and an item into units: kItemUnits for
 // its beginning and end (queries, first loads and results take about as long as
-// three stages) and one per stage of 64 cache rows. Workgroup w of W takes units
+// five stages) and one per stage of 64 cache rows. Workgroup w of W takes units
 // [w T / W, (w + 1) T / W) of all T, so ragged contexts leave every CU the same
 // share, whatever the host knew of the lengths. An item whose stages lie inside
 // one workgroup's range is finished there; of the others each workgroup with
 // some of the stages leaves a part (maximum, sum, unnormalised output) in one of
 // its two places: the second where it has the item's first stage, else the first
 // (a range has at most one of each).
-constexpr int kItemUnits = 3;
+constexpr int kItemUnits = 5;
 __device__ __forceinline__ int item_blocks(const TreeArgs &a, const TreeRequest &r) {
   return (r.nodes * (a.heads / a.kv_heads) + kBlockVectors - 1) / kBlockVectors;
 }
@@ -261,6 +261,18 @@ __global__ __launch_bounds__(64 * kTreeWaves) Q35_WAVES_PER_EU(2) void tree_atte
     const bool active = group < groups;
     const int mg = m0 + kGroupVectors * group;
 
+    // the lane's query vector (spare lanes repeat the last one and store nothing),
+    // asked for before the pages are waited for
+    const int m = min(mg + col, vectors - 1), node = m / qpk, u = m - node * qpk;
+    const size_t head = static_cast<size_t>(rq.row0 + node) * a.heads + g * qpk + u;
+    const uint64_t *words = a.masks + static_cast<size_t>(rq.row0 + node) * a.mask_words;
+    q35_f32x4 raw[KS][2];
+#pragma unroll
+    for (int kk = 0; kk < KS; ++kk)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) raw[kk][i] = *reinterpret_cast<const q35_f32x4 *>(a.q + head * HD + 8 * quad + 32 * kk + 4 * i);
+    q35_compiler_fence();
+
     const int32_t *table = a.page_table + static_cast<size_t>(b) * a.max_pages;
     // The cache rows of the stages, a run of kRowStages at a time (a token per
     // thread): token `tid` of run c (past the request: its stage's first), its
@@ -293,27 +305,16 @@ __global__ __launch_bounds__(64 * kTreeWaves) Q35_WAVES_PER_EU(2) void tree_atte
     lds_barrier();
     issue(s0);
 
-    // the lane's query vector (spare lanes repeat the last one and store nothing)
-    const int m = min(mg + col, vectors - 1), node = m / qpk, u = m - node * qpk;
-    const size_t head = static_cast<size_t>(rq.row0 + node) * a.heads + g * qpk + u;
-    const uint64_t *words = a.masks + static_cast<size_t>(rq.row0 + node) * a.mask_words;
     q35_f16x8 qhi[KS], qlo[KS];
     float sscale;
     {
       // the vector as two binary16 operands: 22 bits under its largest value,
       // which a power of two brings to 2^8 (exact, and any fp32 size fits)
-      // (read twice, for the maximum and for the operands: the vector itself
-      // would take another 64 registers)
-      const float *src = a.q + head * HD + 8 * quad;
       float top = 0.0F;
 #pragma unroll
-      for (int kk = 0; kk < KS; ++kk) {
-        const q35_f32x4 lo = *reinterpret_cast<const q35_f32x4 *>(src + 32 * kk);
-        const q35_f32x4 hi = *reinterpret_cast<const q35_f32x4 *>(src + 32 * kk + 4);
+      for (int kk = 0; kk < KS; ++kk)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) top = fmaxf(top, fmaxf(fabsf(lo[i]), fabsf(hi[i])));
-      }
-      q35_compiler_fence();
+        for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(raw[kk][i >> 2][i & 3]));
       top = q35_max_rows(top);
       int ex = static_cast<int>(__float_as_uint(top) >> 23);  // biased
       ex = ex == 0 || ex == 255 ? 127 + 8 : max(ex, 20);
@@ -323,14 +324,9 @@ __global__ __launch_bounds__(64 * kTreeWaves) Q35_WAVES_PER_EU(2) void tree_atte
       if (a.scale < 0.0F) down = -down;  // the scores' order is then that of the products
 #pragma unroll
       for (int kk = 0; kk < KS; ++kk) {
-        const q35_f32x4 lo = *reinterpret_cast<const q35_f32x4 *>(src + 32 * kk);
-        const q35_f32x4 hi = *reinterpret_cast<const q35_f32x4 *>(src + 32 * kk + 4);
         float x[8];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          x[i] = lo[i] * down;
-          x[4 + i] = hi[i] * down;
-        }
+        for (int i = 0; i < 8; ++i) x[i] = raw[kk][i >> 2][i & 3] * down;
         q35_split_f16(x, qhi[kk], qlo[kk]);
       }
     }
@@ -345,9 +341,11 @@ __global__ __launch_bounds__(64 * kTreeWaves) Q35_WAVES_PER_EU(2) void tree_atte
     // weight of 0.)
     auto tile = [&](int kb, const int *at, int t) {
       const uint32_t lost = static_cast<uint32_t>(q35_ballot(at[lane & 31] < 0));
-      q35_f32x4 s[2];
+      // (the two parts of the queries in sums of their own: four chains of
+      // products that do not wait for each other)
+      q35_f32x4 s[2], low[2];
 #pragma unroll
-      for (int k = 0; k < 2; ++k) s[k] = q35_f32x4{0.0F, 0.0F, 0.0F, 0.0F};
+      for (int k = 0; k < 2; ++k) s[k] = low[k] = q35_f32x4{0.0F, 0.0F, 0.0F, 0.0F};
       int krow[2];
 #pragma unroll
       for (int k = 0; k < 2; ++k) krow[k] = kb + (16 * k + col) * HD + 8 * (quad ^ ((16 * k + col) & (PIECES - 1)));
@@ -360,8 +358,10 @@ __global__ __launch_bounds__(64 * kTreeWaves) Q35_WAVES_PER_EU(2) void tree_atte
 #pragma unroll
         for (int k = 0; k < 2; ++k) s[k] = Q35_MFMA_F32_16X16X32_F16(x[k], qhi[kk], s[k]);
 #pragma unroll
-        for (int k = 0; k < 2; ++k) s[k] = Q35_MFMA_F32_16X16X32_F16(x[k], qlo[kk], s[k]);
+        for (int k = 0; k < 2; ++k) low[k] = Q35_MFMA_F32_16X16X32_F16(x[k], qlo[kk], low[k]);
       }
+#pragma unroll
+      for (int k = 0; k < 2; ++k) s[k] += low[k];
       if (t + kTileTokens > rq.context || lost != 0u) {
         const uint32_t seen = tree_visible(words, a.mask_words, t, rq.context, rq.len);
 #pragma unroll
@@ -396,12 +396,18 @@ __global__ __launch_bounds__(64 * kTreeWaves) Q35_WAVES_PER_EU(2) void tree_atte
       // dims 16 n .. + 15 of row r: pair n of pieces, at that number xor r
       const int r = 4 * quad + (col >> 2), vrow = kb + BLOCK + r * HD + 16 * (r & (PIECES / 2 - 1)) + 4 * (col & 3);
 #pragma unroll
-      for (int n = 0; n < NV; ++n) {
-        const uint16_t *v = cache + (vrow ^ (16 * n));
-        const q35_u32x2 lo = q35_lds_read_tr16(v), hi = q35_lds_read_tr16(v + 16 * HD);
-        const q35_f16x8 x = q35_f16x8_bits(q35_u32x4{lo[0], lo[1], hi[0], hi[1]});
-        acc[n] = Q35_MFMA_F32_16X16X32_F16(x, phi, acc[n]);
-        acc[n] = Q35_MFMA_F32_16X16X32_F16(x, plo, acc[n]);
+      for (int n0 = 0; n0 < NV; n0 += 4) {  // (four at a time: no product waits for the one before)
+        q35_f16x8 x[4];
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          const uint16_t *v = cache + (vrow ^ (16 * (n0 + n)));
+          const q35_u32x2 lo = q35_lds_read_tr16(v), hi = q35_lds_read_tr16(v + 16 * HD);
+          x[n] = q35_f16x8_bits(q35_u32x4{lo[0], lo[1], hi[0], hi[1]});
+        }
+#pragma unroll
+        for (int n = 0; n < 4; ++n) acc[n0 + n] = Q35_MFMA_F32_16X16X32_F16(x[n], phi, acc[n0 + n]);
+#pragma unroll
+        for (int n = 0; n < 4; ++n) acc[n0 + n] = Q35_MFMA_F32_16X16X32_F16(x[n], plo, acc[n0 + n]);
       }
     };
 
