@@ -84,16 +84,18 @@ __device__ __forceinline__ uint32_t tree_visible(const uint64_t *words, int word
 
 // Four dims of an output: normalised by the sum l -- a zero sum saw nothing --
 // and gated.
-__device__ __forceinline__ void tree_store(float *dst, q35_f32x4 y, float l, const float *gates) {
+__device__ __forceinline__ void tree_store(float *dst, q35_f32x4 y, float l, bool gated, q35_f32x4 gate) {
   const float inv = 1.0F / (l == 0.0F ? 1.0F : l);
-  q35_f32x4 gate = {0.0F, 0.0F, 0.0F, 0.0F};
-  if (gates != nullptr) gate = *reinterpret_cast<const q35_f32x4 *>(gates);
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     y[e] *= inv;
-    if (gates != nullptr) y[e] *= sigmoid_stable(gate[e]);
+    if (gated) y[e] *= sigmoid_stable(gate[e]);
   }
   *reinterpret_cast<q35_f32x4 *>(dst) = y;
+}
+
+__device__ __forceinline__ q35_f32x4 tree_gate(const float *gates, size_t at) {
+  return gates != nullptr ? *reinterpret_cast<const q35_f32x4 *>(gates + at) : q35_f32x4{0.0F, 0.0F, 0.0F, 0.0F};
 }
 
 // The work is cut into items (request, KV head, block of up to 128 query
@@ -159,7 +161,7 @@ __device__ void tree_row_by_row(const TreeArgs &a, const TreeRequest &rq, int i,
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[e] = fmaf(p, half_bits_to_float(a.v_pool[at + e]), o[e] * keep);
   }
-  tree_store(a.out + head, o, l, a.gates != nullptr ? a.gates + head : nullptr);
+  tree_store(a.out + head, o, l, a.gates != nullptr, tree_gate(a.gates, head));
 }
 
 // One workgroup of eight wavefronts. A stage's K and V rows go straight from
@@ -499,7 +501,7 @@ __global__ __launch_bounds__(64 * kTreeWaves) Q35_WAVES_PER_EU(2) void tree_atte
         if (whole) {
           const int vn = (m0 + v) / qpk, vu = m0 + v - vn * qpk;
           const size_t to = (static_cast<size_t>(rq.row0 + vn) * a.heads + g * qpk + vu) * HD + 4 * f;
-          tree_store(a.out + to, y, sh.stat[v / kGroupVectors][1][v & (kGroupVectors - 1)], a.gates != nullptr ? a.gates + to : nullptr);
+          tree_store(a.out + to, y, sh.stat[v / kGroupVectors][1][v & (kGroupVectors - 1)], a.gates != nullptr, tree_gate(a.gates, to));
         } else {
           *reinterpret_cast<q35_f32x4 *>(a.part_o + (place + v) * HD + 4 * f) = y;
         }
@@ -536,13 +538,23 @@ __global__ __launch_bounds__(64) void tree_merge_kernel(TreeArgs a) {
   if (w0 == w1) return;  // finished by its workgroup
   const size_t at = m % kBlockVectors;
   auto place = [&](int w) { return (2 * static_cast<size_t>(w) + (w == w0 ? 1 : 0)) * kBlockVectors + at; };
-  // 64 parts at a time: a part's maximum and sum per lane
-  float top = -INFINITY;
+  // 64 parts at a time, a part's maximum and sum per lane; the first parts' rows
+  // and the gates are asked for together with the first of those
+  constexpr int U = 4;  // parts' rows in flight
+  const size_t head = (static_cast<size_t>(rq.row0 + i) * a.heads + h) * HD + 4 * f;
+  q35_f32x4 x[U];
+  auto ask = [&](int first_part) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) x[u] = *reinterpret_cast<const q35_f32x4 *>(a.part_o + place(min(first_part + u, w1)) * HD + 4 * f);
+  };
+  q35_f32x2 ml = *reinterpret_cast<const q35_f32x2 *>(a.part_ml + 2 * place(min(w0 + lane, w1)));
   bool special = false;
-  for (int w = w0 + lane; w <= w1; w += 64) {
-    top = fmaxf(top, a.part_ml[2 * place(w)]);
-    special |= a.specials[2 * w + (w == w0 ? 1 : 0)] != 0;
-  }
+  for (int w = w0 + lane; w <= w1; w += 64) special |= a.specials[2 * w + (w == w0 ? 1 : 0)] != 0;
+  ask(w0);
+  const q35_f32x4 gate = tree_gate(a.gates, head);
+  q35_compiler_fence();
+  float top = ml[0];
+  for (int w = w0 + lane + 64; w <= w1; w += 64) top = fmaxf(top, a.part_ml[2 * place(w)]);
   top = group_max<64>(top);
   if (q35_ballot(special) != 0ull) {
     tree_row_by_row<HD>(a, rq, i, h, b);
@@ -553,18 +565,11 @@ __global__ __launch_bounds__(64) void tree_merge_kernel(TreeArgs a) {
   float l = 0.0F;
   for (int c = w0; c <= w1; c += 64) {
     const int n = min(64, w1 - c + 1);
-    float weight = 0.0F, lw = 0.0F;
-    if (lane < n) {
-      const q35_f32x2 ml = *reinterpret_cast<const q35_f32x2 *>(a.part_ml + 2 * place(c + lane));
-      weight = Q35_EXP2(ml[0] - least);
-      lw = ml[1] * weight;
-    }
-    l += group_sum<64>(lw);
-    constexpr int U = 8;  // parts in flight
+    if (c > w0) ml = *reinterpret_cast<const q35_f32x2 *>(a.part_ml + 2 * place(min(c + lane, w1)));
+    const float weight = lane < n ? Q35_EXP2(ml[0] - least) : 0.0F;
+    l += group_sum<64>(lane < n ? ml[1] * weight : 0.0F);
     for (int k = 0; k < n; k += U) {
-      q35_f32x4 x[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u) x[u] = *reinterpret_cast<const q35_f32x4 *>(a.part_o + place(c + min(k + u, n - 1)) * HD + 4 * f);
+      if (c + k > w0) ask(c + k);
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         if (k + u >= n) break;
@@ -574,8 +579,7 @@ __global__ __launch_bounds__(64) void tree_merge_kernel(TreeArgs a) {
       }
     }
   }
-  const size_t head = (static_cast<size_t>(rq.row0 + i) * a.heads + h) * HD + 4 * f;
-  tree_store(a.out + head, o, l, a.gates != nullptr ? a.gates + head : nullptr);
+  tree_store(a.out + head, o, l, a.gates != nullptr, gate);
 }
 
 // ------------------------------------------------------------- acceptance
