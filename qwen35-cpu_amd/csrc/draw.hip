@@ -15,12 +15,15 @@
 // tokens fits 64 bits.
 //
 //   slices: one workgroup per 4096 tokens of a row, which it reads once into
-//     registers; counts and weights of its tokens per quarter octave of weight
-//     below its own largest (bins on a grid common to the row), and the keys
-//     of its topmost bins, bin by bin.
+//     registers; counts of its tokens per quarter octave of weight below its own
+//     largest (bins on a grid common to the row), the bins' weights, and the
+//     tokens of its topmost bins, bin by bin.
 //   pick: one workgroup per row joins the slices' bins, finds the bin that
 //     each cut falls in, and settles it among that bin's keys -- from the
 //     slices' lists, or from the logits where a list does not reach that far.
+// Rows with a small top-k ("light") need no weight below its cut: their slices
+// leave out the exponentials, and the pick gathers all keys through the cut's
+// bin once.
 #include "q35_device.h"
 #include "q35_internal.h"
 
@@ -28,11 +31,15 @@ namespace q35 {
 namespace {
 
 constexpr int kSliceThreads = 256, kSlicePer = 16, kSliceTokens = kSliceThreads * kSlicePer;
-constexpr int kBins = 192;   // quarter octaves: a weight below 2^-44 is no whole number left
-constexpr int kListed = 256; // keys a slice lists
+constexpr int kBins = 192;    // quarter octaves: a weight below 2^-44 is no whole number left
+constexpr int kListed = 1024; // tokens a slice lists
+constexpr int kLightTopK = 512;
+constexpr int kUnitBits = 43;
 constexpr double kUnit = 8796093022208.0;  // 2^43
 constexpr int kPickThreads = 1024, kPickWaves = kPickThreads / 64;
-constexpr int kSettle = 256; // keys settled by comparing each with each
+constexpr int kParts = kPickThreads;  // parts that a bin of many keys is split into
+constexpr int kSettle = 256;          // keys settled by comparing each with each
+constexpr int kCached = 2048;         // keys of a light row kept in LDS
 constexpr int kMaxSlices = kDrawMaxVocab / kSliceTokens;
 
 struct DrawOptions {
@@ -40,17 +47,21 @@ struct DrawOptions {
   float bin_scale; // bins per unit of x
   int top_k;       // 0: all
   float top_p, min_p;
+  bool light;
 };
 
 __device__ __forceinline__ DrawOptions draw_options(const DrawArgs &a, int r) {
   DrawOptions o;
   const float t = a.temperatures != nullptr ? a.temperatures[r] : 1.0F;
+  const int k = a.top_k != nullptr ? a.top_k[r] : 0;
+  const float p = a.top_p != nullptr ? a.top_p[r] : 1.0F, m = a.min_p != nullptr ? a.min_p[r] : 0.0F;
   const bool greedy = !(t > 1.0e-6F);  // the largest logit, as a draw from the first token alone
   o.inv_t = 1.4426950408889634074 / (greedy ? 1.0 : static_cast<double>(t));
   o.bin_scale = fminf(fmaxf(static_cast<float>(4.0 * o.inv_t), 1.0e-30F), 1.0e30F);
-  o.top_k = greedy ? 1 : a.top_k != nullptr ? max(a.top_k[r], 0) : 0;
-  o.top_p = greedy || a.top_p == nullptr ? 1.0F : a.top_p[r];
-  o.min_p = greedy || a.min_p == nullptr ? 0.0F : a.min_p[r];
+  o.top_k = greedy ? 1 : max(k, 0);
+  o.top_p = greedy ? 1.0F : p;
+  o.min_p = greedy ? 0.0F : m;
+  o.light = o.top_k > 0 && o.top_k <= kLightTopK;
   return o;
 }
 
@@ -70,10 +81,28 @@ __device__ __forceinline__ int bins_below(float top, float y) {
 __device__ __forceinline__ double draw_power(float x, float top, double inv_t) {
   return (static_cast<double>(x) - static_cast<double>(top)) * inv_t;
 }
+// 2^z in units of 2^-43, to the nearest whole number (z <= 0): 2^z = 2^n e^r with
+// |r| <= ln(2) / 2, e^r by its series through r^11 (the rest is below 2^-47), and
+// the rounding by an addition of 2^52, whose sum holds the number in its low bits.
 __device__ __forceinline__ unsigned long long draw_weight(float x, float top, double inv_t) {
-  if (x == top) return static_cast<unsigned long long>(kUnit);
+  if (x == top) return 1ull << kUnitBits;
   const double z = draw_power(x, top, inv_t);
-  return z > -45.0 ? static_cast<unsigned long long>(exp2(z) * kUnit + 0.5) : 0ull;
+  if (!(z > -45.0)) return 0ull;
+  const double n = rint(z), r = (z - n) * 0.69314718055994530942;
+  double e = 1.0 / 39916800.0;
+  e = fma(e, r, 1.0 / 3628800.0);
+  e = fma(e, r, 1.0 / 362880.0);
+  e = fma(e, r, 1.0 / 40320.0);
+  e = fma(e, r, 1.0 / 5040.0);
+  e = fma(e, r, 1.0 / 720.0);
+  e = fma(e, r, 1.0 / 120.0);
+  e = fma(e, r, 1.0 / 24.0);
+  e = fma(e, r, 1.0 / 6.0);
+  e = fma(e, r, 0.5);
+  e = fma(e, r, 1.0);
+  e = fma(e, r, 1.0);
+  const double w = ldexp(e, static_cast<int>(n) + kUnitBits) + 4503599627370496.0;
+  return static_cast<unsigned long long>(__double_as_longlong(w)) & 0xfffffffffffffull;
 }
 
 // ---------------------------------------------------------------- slices
@@ -118,11 +147,13 @@ __global__ __launch_bounds__(kSliceThreads) void draw_slices_kernel(DrawArgs a, 
     if (x[i] == -INFINITY) continue;
     const int bin = bins_below(ytop, bin_floor(x[i], o.bin_scale));
     atomicAdd(&number[bin], 1u);
-    const unsigned long long m = draw_weight(x[i], top, o.inv_t);
-    if (m != 0ull) atomicAdd(&mass[bin], m);
+    if (!o.light) {
+      const unsigned long long m = draw_weight(x[i], top, o.inv_t);
+      if (m != 0ull) atomicAdd(&mass[bin], m);
+    }
   }
   __syncthreads();
-  if (tid < kBins) w.mass[at * kBins + tid] = mass[tid];
+  if (tid < kBins && !o.light) w.mass[at * kBins + tid] = mass[tid];
   // inclusive counts over the bins: three bins per lane of the first wavefront
   if (tid < 64) {
     unsigned n[3];
@@ -141,8 +172,10 @@ __global__ __launch_bounds__(kSliceThreads) void draw_slices_kernel(DrawArgs a, 
     for (int e = 0; e < 3; ++e) {
       const unsigned end = before + n[e];
       w.ends[at * kBins + 3 * lane + e] = static_cast<uint16_t>(end);
-      // the bin's first place in the list, where the list holds all of it
-      number[3 * lane + e] = end <= kListed ? (e == 0 ? before : before + n[e - 1]) : 0x80000000u;
+      // the bin's first place in the list, where the list holds all of it (and
+      // some of it may be among the first top_k)
+      const unsigned first = e == 0 ? before : before + n[e - 1];
+      number[3 * lane + e] = end <= kListed && !(o.light && first >= static_cast<unsigned>(o.top_k)) ? first : 0x80000000u;
     }
   }
   __syncthreads();
@@ -152,23 +185,26 @@ __global__ __launch_bounds__(kSliceThreads) void draw_slices_kernel(DrawArgs a, 
     const int bin = bins_below(ytop, bin_floor(x[i], o.bin_scale));
     if ((number[bin] & 0x80000000u) != 0u) continue;
     const unsigned place = atomicAdd(&number[bin], 1u);
-    w.list[at * kListed + place] = argmax_key(x[i], static_cast<uint32_t>(t0 + tid + i * kSliceThreads));
+    w.list[at * kListed + place] = static_cast<uint16_t>(tid + i * kSliceThreads);
   }
 }
 
 // ------------------------------------------------------------------ pick
 struct PickShared {
   float top[kMaxSlices];
-  int below[kMaxSlices];           // bins from the row's top bin to the slice's
-  int first[kMaxSlices], end[kMaxSlices];  // the places of a bin's keys in each slice's list
-  unsigned long long mass[kBins];  // running weight through each bin
-  unsigned number[kBins];          // running count
-  unsigned long long sub_mass[kSettle], key[kSettle];
-  unsigned sub_number[kSettle];
+  int below[kMaxSlices];                   // bins from the row's top bin to the slice's
+  int first[kMaxSlices], end[kMaxSlices];  // the places of a bin's (or of several bins') tokens in each slice's list
+  unsigned long long mass[kBins];          // running weight through each bin
+  unsigned number[kBins];                  // running count
+  unsigned long long part_mass[kParts], cache[kCached];
+  unsigned part_number[kParts];
+  unsigned long long key[kSettle], weight[kSettle];
   float wave_top[kPickWaves];
+  unsigned long long wave_mass[kPickWaves];
+  unsigned wave_number[kPickWaves];
   unsigned found;
   int where;
-  unsigned long long low, high, result_key, result_mass;
+  unsigned long long result_key, result_mass;
 };
 
 enum : int { kByCount = 0, kByMass = 1, kByKey = 2 };
@@ -182,25 +218,110 @@ struct Picker {
   float top, ytop, penalty;
   const float *logits;
   const int32_t *counts;
+  int cached = -1;  // keys in sh.cache, those of the bins through cached_bin (-1: none)
+  int cached_bin = -1;
 
-  // f(key) for every key of bin g, from the places in sh.first / sh.end
+  __device__ __forceinline__ int bin_at(float x) const { return bins_below(ytop, bin_floor(x, o.bin_scale)); }
+
+  // The list places of bins g0 .. g1 in every slice (then a barrier).
+  __device__ __forceinline__ void places(int g0, int g1) const {
+    for (int s = threadIdx.x; s < slices; s += kPickThreads) {
+      int first = 0, end = 0;
+      // the slice's bins: its own bin b is the row's b + below, the last takes
+      // all that lies further down
+      const int b0 = max(g0 - sh.below[s], 0), b1 = g1 == kBins - 1 ? kBins - 1 : g1 - sh.below[s];
+      if (sh.top[s] != -INFINITY && b1 >= 0 && (g1 == kBins - 1 || g0 - sh.below[s] < kBins - 1)) {
+        const uint16_t *ends = w.ends + (static_cast<size_t>(r) * w.slices + s) * kBins;
+        // (a slice's last bin holds bins of the row beyond g1 too, so a range that
+        // ends in it, short of the row's last, takes only what lies before)
+        const int last = g1 == kBins - 1 ? kBins - 1 : min(b1, kBins - 2);
+        first = b0 > 0 ? ends[b0 - 1] : 0;
+        end = ends[last];
+      }
+      sh.first[s] = first;
+      sh.end[s] = max(first, end);
+    }
+    __syncthreads();
+  }
+  // f(key) for every key of bins g0 .. g1, from the places in sh.first / sh.end
   template <typename F>
-  __device__ __forceinline__ void for_each(int g, F f) const {
+  __device__ __forceinline__ void for_each(int g0, int g1, F f) const {
+    if (cached >= 0 && g1 <= cached_bin) {
+      for (int e = threadIdx.x; e < cached; e += kPickThreads) {
+        const unsigned long long k = sh.cache[e];
+        const int bin = bin_at(argmax_key_value(k));
+        if (bin >= g0 && bin <= g1) f(k);
+      }
+      return;
+    }
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     for (int s = wave; s < slices; s += kPickWaves) {
-      const int first = sh.first[s], end = sh.end[s];
+      const int first = sh.first[s], end = sh.end[s], t0 = s * kSliceTokens;
       if (first >= end) continue;
-      if (end <= kListed) {
-        const unsigned long long *list = w.list + (static_cast<size_t>(r) * w.slices + s) * kListed;
-        for (int e = first + lane; e < end; e += 64) f(list[e]);
+      if (end <= kListed && !(o.light && first >= o.top_k)) {
+        const uint16_t *list = w.list + (static_cast<size_t>(r) * w.slices + s) * kListed;
+        for (int e = first + lane; e < end; e += 64) {
+          const int t = t0 + list[e];
+          f(argmax_key(draw_value(logits[t], counts != nullptr ? counts[t] : 0, penalty), static_cast<uint32_t>(t)));
+        }
       } else {
-        const int t1 = min(a.vocab, (s + 1) * kSliceTokens);
-        for (int t = s * kSliceTokens + lane; t < t1; t += 64) {
-          const float x = draw_value(logits[t], counts != nullptr ? counts[t] : 0, penalty);
-          if (x != -INFINITY && bins_below(ytop, bin_floor(x, o.bin_scale)) == g) f(argmax_key(x, static_cast<uint32_t>(t)));
+        constexpr int U = 8;
+        for (int e = lane; e < kSliceTokens && t0 + e < a.vocab; e += 64 * U) {
+          float x[U];
+          int seen[U];
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            const int t = min(t0 + e + 64 * u, a.vocab - 1);
+            x[u] = logits[t];
+            seen[u] = counts != nullptr ? counts[t] : 0;
+          }
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            const int t = t0 + e + 64 * u;
+            const float v = draw_value(x[u], seen[u], penalty);
+            if (e + 64 * u >= kSliceTokens || t >= a.vocab || v == -INFINITY) continue;
+            const int bin = bin_at(v);
+            if (bin >= g0 && bin <= g1) f(argmax_key(v, static_cast<uint32_t>(t)));
+          }
         }
       }
     }
+  }
+
+  // Inclusive sums of the threads' (m, c) in thread order.
+  __device__ __forceinline__ void running(unsigned long long &m, unsigned &c) const {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const unsigned long long um = __shfl(m, max(lane - d, 0), 64);
+      const unsigned uc = __shfl(c, max(lane - d, 0), 64);
+      if (lane >= d) {
+        m += um;
+        c += uc;
+      }
+    }
+    if (lane == 63) {
+      sh.wave_mass[wave] = m;
+      sh.wave_number[wave] = c;
+    }
+    __syncthreads();
+    for (int v = 0; v < wave; ++v) {
+      m += sh.wave_mass[v];
+      c += sh.wave_number[v];
+    }
+  }
+  // sh.mass / sh.number from each bin's own to running sums
+  __device__ __forceinline__ void running_bins() const {
+    const int tid = threadIdx.x;
+    __syncthreads();
+    unsigned long long m = tid < kBins ? sh.mass[tid] : 0ull;
+    unsigned c = tid < kBins ? sh.number[tid] : 0u;
+    running(m, c);
+    if (tid < kBins) {
+      sh.mass[tid] = m;
+      sh.number[tid] = c;
+    }
+    __syncthreads();
   }
 
   // The position in bin g at which the running count or weight reaches
@@ -212,89 +333,65 @@ struct Picker {
     unsigned above = g > 0 ? sh.number[g - 1] : 0u;
     int n = static_cast<int>(sh.number[g] - above);
     __syncthreads();  // the last settle's readers are done
-    for (int s = tid; s < slices; s += kPickThreads) {
-      int first = 0, end = 0;
-      const int bin = g - sh.below[s];
-      if (sh.top[s] != -INFINITY && (g == kBins - 1 || (bin >= 0 && bin < kBins - 1))) {
-        const uint16_t *ends = w.ends + (static_cast<size_t>(r) * w.slices + s) * kBins;
-        const int b0 = max(bin, 0), b1 = g == kBins - 1 ? kBins - 1 : bin;  // the last bin takes all below it
-        first = b0 > 0 ? ends[b0 - 1] : 0;
-        end = ends[b1];
-      }
-      sh.first[s] = first;
-      sh.end[s] = end;
-    }
-    if (tid == 0) {
-      sh.low = ~0ull;
-      sh.high = 0ull;
-    }
-    __syncthreads();
+    if (!(cached >= 0 && g <= cached_bin)) places(g, g);
     unsigned long long low = 0ull, high = ~0ull;
-    if (n > kSettle) {
-      for_each(g, [&](unsigned long long k) {
-        atomicMin(&sh.low, k);
-        atomicMax(&sh.high, k);
-      });
-      __syncthreads();
-      low = sh.low;
-      high = sh.high;
+    if (n > kSettle && g < kBins - 1) {
+      // keys of values whose x * scale may round into the bin
+      const float y = ytop - static_cast<float>(g), x0 = y / o.bin_scale, x1 = (y + 1.0F) / o.bin_scale;
+      const float lo = x0 - fabsf(x0) * 1.0e-6F, hi = x1 + fabsf(x1) * 1.0e-6F;
+      if (lo > -INFINITY && lo < hi && hi < INFINITY) {
+        low = argmax_key(lo, 0xffffffffu);
+        high = argmax_key(hi, 0u);
+      }
     }
     while (n > kSettle) {  // the range shrinks every turn: keys differ, so n reaches 1 at the latest
-      const int bits = 64 - __builtin_clzll(high - low), shift = max(0, bits - 8);
-      if (tid < kSettle) {
-        sh.sub_mass[tid] = 0ull;
-        sh.sub_number[tid] = 0u;
-      }
+      const int shift = max(0, 54 - __builtin_clzll(high - low));
+      sh.part_mass[tid] = 0ull;
+      sh.part_number[tid] = 0u;
       if (tid == 0) sh.where = -1;
       __syncthreads();
-      for_each(g, [&](unsigned long long k) {
+      for_each(g, g, [&](unsigned long long k) {
         if (k < low || k > high) return;
-        const int e = kSettle - 1 - static_cast<int>((k - low) >> shift);  // descending
-        atomicAdd(&sh.sub_number[e], 1u);
+        const int e = kParts - 1 - static_cast<int>((k - low) >> shift);  // descending
+        atomicAdd(&sh.part_number[e], 1u);
         const unsigned long long m = draw_weight(argmax_key_value(k), top, o.inv_t);
-        if (m != 0ull) atomicAdd(&sh.sub_mass[e], m);
+        if (m != 0ull) atomicAdd(&sh.part_mass[e], m);
       });
       __syncthreads();
       // running sums of the parts up to each, and the part to go on in
-      unsigned long long m = 0ull;
-      unsigned c = 0u;
-      if (tid < kSettle) {
-        for (int e = 0; e <= tid; ++e) {
-          m += sh.sub_mass[e];
-          c += sh.sub_number[e];
-        }
-        const unsigned long long m0 = m - sh.sub_mass[tid];
-        const unsigned c0 = c - sh.sub_number[tid];
-        bool here;
-        if (mode == kByCount) {
-          here = above + c >= target && above + c0 < target;
-        } else if (mode == kByMass) {
-          here = before + m >= target && before + m0 < target;
-        } else {
-          const unsigned long long k = target < low ? low : target > high ? high : target;
-          here = tid == kSettle - 1 - static_cast<int>((k - low) >> shift);
-        }
-        if (here) sh.where = tid;
+      const unsigned long long own_m = sh.part_mass[tid];
+      const unsigned own_c = sh.part_number[tid];
+      unsigned long long m = own_m;
+      unsigned c = own_c;
+      running(m, c);
+      bool here;
+      if (mode == kByCount) {
+        here = above + c >= target && above + c - own_c < target;
+      } else if (mode == kByMass) {
+        here = before + m >= target && before + m - own_m < target;
+      } else {
+        const unsigned long long k = target < low ? low : target > high ? high : target;
+        here = tid == kParts - 1 - static_cast<int>((k - low) >> shift);
       }
+      sh.part_mass[tid] = m;
+      sh.part_number[tid] = c;
+      if (here) sh.where = tid;
       __syncthreads();
       int e = sh.where;
       if (e < 0) {  // the keys' weights round to less than their bin's sum: the last part that weighs, or has keys
-        bool weighs = false;
-        for (int i = 0; i < kSettle; ++i) {
-          if (sh.sub_mass[i] != 0ull || (!weighs && sh.sub_number[i] != 0u)) e = i;
-          weighs = weighs || sh.sub_mass[i] != 0ull;
+        const bool weighs = sh.part_mass[kParts - 1] != 0ull;
+        for (int i = 0; i < kParts; ++i) {
+          const bool more = weighs ? sh.part_mass[i] != (i > 0 ? sh.part_mass[i - 1] : 0ull)
+                                   : sh.part_number[i] != (i > 0 ? sh.part_number[i - 1] : 0u);
+          if (more) e = i;
         }
       }
-      unsigned long long m1 = 0ull;
-      unsigned c1 = 0u;
-      for (int i = 0; i < e; ++i) {
-        m1 += sh.sub_mass[i];
-        c1 += sh.sub_number[i];
-      }
-      before += m1;
-      above += c1;
-      n = static_cast<int>(sh.sub_number[e]);
-      low += static_cast<unsigned long long>(kSettle - 1 - e) << shift;
+      const unsigned long long m0 = e > 0 ? sh.part_mass[e - 1] : 0ull;
+      const unsigned c0 = e > 0 ? sh.part_number[e - 1] : 0u;
+      before += m0;
+      above += c0;
+      n = static_cast<int>(sh.part_number[e] - c0);
+      low += static_cast<unsigned long long>(kParts - 1 - e) << shift;
       const unsigned long long last = low + ((1ull << shift) - 1ull);
       high = last < high ? last : high;
       __syncthreads();
@@ -306,11 +403,11 @@ struct Picker {
       sh.result_mass = before;
     }
     __syncthreads();
-    for_each(g, [&](unsigned long long k) {
+    for_each(g, g, [&](unsigned long long k) {
       if (k < low || k > high) return;
       const unsigned i = atomicAdd(&sh.found, 1u);
       sh.key[i] = k;
-      sh.sub_mass[i] = draw_weight(argmax_key_value(k), top, o.inv_t);
+      sh.weight[i] = draw_weight(argmax_key_value(k), top, o.inv_t);
     });
     __syncthreads();
     const int i = tid >> 2, q = tid & 3;
@@ -319,7 +416,7 @@ struct Picker {
     unsigned c = 0u;
     for (int e = q; e < n; e += 4) {
       if (sh.key[e] >= mine) {
-        m += sh.sub_mass[e];
+        m += sh.weight[e];
         ++c;
       }
     }
@@ -328,7 +425,7 @@ struct Picker {
       m += __shfl_xor(m, d, 64);
       c += __shfl_xor(c, d, 64);
     }
-    const unsigned long long own = i < n ? sh.sub_mass[i] : 0ull;
+    const unsigned long long own = i < n ? sh.weight[i] : 0ull;
     // without a key that meets the condition: the last one that weighs (as above)
     if (q == 0 && i < n && mode == kByMass && own != 0ull) atomicMax(&sh.result_mass, before + m);
     __syncthreads();
@@ -355,7 +452,7 @@ struct Picker {
   }
 
   // The first bin whose running count or weight reaches the target (the last
-  // bin that holds some, where rounding leaves none).
+  // bin, where rounding leaves none).
   __device__ int bin_of(int mode, unsigned long long target) const {
     const int tid = threadIdx.x;
     __syncthreads();
@@ -368,6 +465,34 @@ struct Picker {
     }
     __syncthreads();
     return sh.where;
+  }
+
+  // A light row: the weights of the bins through g, and their keys where they
+  // are not too many (the bins beyond hold none).
+  __device__ __forceinline__ void weigh(int g) {
+    const int tid = threadIdx.x, n = static_cast<int>(sh.number[g]);
+    __syncthreads();
+    if (tid < kBins) sh.mass[tid] = 0ull;
+    if (tid == 0) sh.found = 0u;
+    places(0, g);
+    const bool keep = n <= kCached;
+    for_each(0, g, [&](unsigned long long k) {
+      const float x = argmax_key_value(k);
+      const unsigned long long m = draw_weight(x, top, o.inv_t);
+      if (m != 0ull) atomicAdd(&sh.mass[bin_at(x)], m);
+      if (keep) sh.cache[atomicAdd(&sh.found, 1u)] = k;
+    });
+    __syncthreads();
+    if (keep) {
+      cached = n;
+      cached_bin = g;
+    }
+    // running weights; the counts are running already
+    unsigned long long m = tid < kBins ? sh.mass[tid] : 0ull;
+    unsigned c = 0u;
+    running(m, c);
+    if (tid < kBins) sh.mass[tid] = m;
+    __syncthreads();
   }
 };
 
@@ -386,6 +511,7 @@ __global__ __launch_bounds__(kPickThreads) void draw_pick_kernel(DrawArgs a, Dra
            penalty,
            a.logits + static_cast<size_t>(r) * a.stride,
            a.counts != nullptr && penalty > 1.0F ? a.counts + static_cast<size_t>(r) * a.vocab : nullptr};
+  const float u = a.uniforms[r];
   // the row's largest value and each slice's distance from it
   float top = -INFINITY;
   for (int s = tid; s < w.slices; s += kPickThreads) {
@@ -413,65 +539,59 @@ __global__ __launch_bounds__(kPickThreads) void draw_pick_kernel(DrawArgs a, Dra
   p.ytop = bin_floor(top, p.o.bin_scale);
   for (int s = tid; s < w.slices; s += kPickThreads) sh.below[s] = bins_below(p.ytop, bin_floor(sh.top[s], p.o.bin_scale));
   __syncthreads();
-  // the slices' bins, weights brought from each slice's largest to the row's
-  for (int e = tid; e < w.slices * kBins; e += kPickThreads) {
-    const int s = e / kBins, bin = e - s * kBins;
+  // the slices' bins, four to a thread, weights brought from each slice's
+  // largest to the row's
+  for (int e = tid; e < w.slices * (kBins / 4); e += kPickThreads) {
+    const int s = e / (kBins / 4), bin = 4 * (e - s * (kBins / 4));
     const float x = sh.top[s];
     if (x == -INFINITY) continue;
     const size_t at = (static_cast<size_t>(r) * w.slices + s) * kBins + bin;
-    const unsigned n = w.ends[at] - (bin > 0 ? w.ends[at - 1] : 0u);
-    if (n == 0u) continue;
-    const int g = min(kBins - 1, sh.below[s] + bin);
-    atomicAdd(&sh.number[g], n);
-    unsigned long long m = w.mass[at];
-    if (x != top) {
-      const double z = draw_power(x, top, p.o.inv_t);
-      m = z > -45.0 ? static_cast<unsigned long long>(static_cast<double>(m) * exp2(z) + 0.5) : 0ull;
+    const q35_u32x2 ends = *reinterpret_cast<const q35_u32x2 *>(w.ends + at);
+    unsigned last = bin > 0 ? w.ends[at - 1] : 0u;
+    const double scale = x == top ? 1.0 : exp2(fmax(draw_power(x, top, p.o.inv_t), -1000.0));
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const unsigned end = (ends[k >> 1] >> (16 * (k & 1))) & 0xffffu, n = end - last;
+      last = end;
+      if (n == 0u) continue;
+      const int g = min(kBins - 1, sh.below[s] + bin + k);
+      atomicAdd(&sh.number[g], n);
+      if (p.o.light) continue;
+      const unsigned long long m = static_cast<unsigned long long>(static_cast<double>(w.mass[at + k]) * scale + 0.5);
+      if (m != 0ull) atomicAdd(&sh.mass[g], m);
     }
-    if (m != 0ull) atomicAdd(&sh.mass[g], m);
   }
-  __syncthreads();
-  {
-    unsigned long long m = 0ull;
-    unsigned n = 0u;
-    if (tid < kBins)
-      for (int e = 0; e <= tid; ++e) {
-        m += sh.mass[e];
-        n += sh.number[e];
-      }
-    __syncthreads();
-    if (tid < kBins) {
-      sh.mass[tid] = m;
-      sh.number[tid] = n;
-    }
-    __syncthreads();
-  }
+  p.running_bins();
   const unsigned total = sh.number[kBins - 1];
+  const int top_k = p.o.top_k > 0 && static_cast<unsigned>(p.o.top_k) < total ? p.o.top_k : 0;
+  if (p.o.light) p.weigh(p.bin_of(kByCount, top_k > 0 ? top_k : total));
   unsigned long long kept = sh.mass[kBins - 1];
-  if (p.o.top_k > 0 && static_cast<unsigned>(p.o.top_k) < total) {
-    p.settle(p.bin_of(kByCount, p.o.top_k), kByCount, p.o.top_k);
+  if (top_k > 0) {
+    p.settle(p.bin_of(kByCount, top_k), kByCount, top_k);
     kept = sh.result_mass;
   }
   unsigned long long cut = kept;
-  if (!(p.o.top_p >= 1.0F)) {
-    const double want = ceil(fmax(static_cast<double>(p.o.top_p), 0.0) * static_cast<double>(kept));
-    unsigned long long target = want < 1.0 ? 1ull : static_cast<unsigned long long>(want);
-    if (target > kept) target = kept;
-    p.settle(p.bin_of(kByMass, target), kByMass, target);
-    cut = sh.result_mass < cut ? sh.result_mass : cut;
-  }
   if (p.o.min_p > 0.0F && top != INFINITY) {
     // the smallest value that weighs min_p, rounded up to fp32
     const double least = static_cast<double>(top) + log2(fmin(static_cast<double>(p.o.min_p), 1.0)) / p.o.inv_t;
     float x = static_cast<float>(least);
     if (static_cast<double>(x) < least) x = nextafterf(x, INFINITY);
     x = fminf(x, top) + 0.0F;
-    if (x > -INFINITY) {
-      p.settle(bins_below(p.ytop, bin_floor(x, p.o.bin_scale)), kByKey, argmax_key(x, 0xffffffffu));
+    const int g = x > -INFINITY ? p.bin_at(x) : kBins - 1;
+    if (x > -INFINITY && (g == 0 || sh.mass[g - 1] < cut)) {  // (else it lies beyond the first top_k)
+      p.settle(g, kByKey, argmax_key(x, 0xffffffffu));
       cut = sh.result_mass < cut ? sh.result_mass : cut;
     }
   }
-  const float u = a.uniforms[r];
+  if (!(p.o.top_p >= 1.0F)) {
+    const double want = ceil(fmax(static_cast<double>(p.o.top_p), 0.0) * static_cast<double>(kept));
+    unsigned long long target = want < 1.0 ? 1ull : static_cast<unsigned long long>(want);
+    if (target > kept) target = kept;
+    if (target < cut) {  // (else it lies beyond the cut there is)
+      p.settle(p.bin_of(kByMass, target), kByMass, target);
+      cut = sh.result_mass < cut ? sh.result_mass : cut;
+    }
+  }
   const double at = floor((u > 0.0F ? static_cast<double>(u) : 0.0) * static_cast<double>(cut));
   unsigned long long target = at >= static_cast<double>(cut) ? cut : static_cast<unsigned long long>(at) + 1ull;
   if (target > cut) target = cut;
@@ -498,7 +618,7 @@ DrawScratch draw_scratch(int rows, int vocab, char *base, size_t *bytes) {
     return p;
   };
   w.mass = reinterpret_cast<unsigned long long *>(take(n * kBins * 8));
-  w.list = reinterpret_cast<unsigned long long *>(take(n * kListed * 8));
+  w.list = reinterpret_cast<uint16_t *>(take(n * kListed * 2));
   w.ends = reinterpret_cast<uint16_t *>(take(n * kBins * 2));
   w.top = reinterpret_cast<float *>(take(n * 4));
   *bytes = at;

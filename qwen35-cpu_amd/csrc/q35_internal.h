@@ -516,8 +516,8 @@ struct DrawArgs {
 };
 struct DrawScratch {  // per row and slice
   int slices = 0;
-  unsigned long long *mass = nullptr, *list = nullptr;
-  uint16_t *ends = nullptr;
+  unsigned long long *mass = nullptr;
+  uint16_t *list = nullptr, *ends = nullptr;
   float *top = nullptr;
 };
 size_t draw_scratch_bytes(int rows, int vocab);

@@ -225,6 +225,7 @@ inline unsigned long long atomicMax(unsigned long long *p, unsigned long long v)
   }
   return cur;
 }
+inline long long __double_as_longlong(double d) { long long v; std::memcpy(&v, &d, 8); return v; }
 inline unsigned __float_as_uint(float f) { unsigned u; std::memcpy(&u, &f, 4); return u; }
 inline int __builtin_amdgcn_readlane(int v, int src) { return ::q35emu::readlane(v, src); }
 // v_perm_b32: byte i of the result is byte sel.byte[i] of the eight bytes
