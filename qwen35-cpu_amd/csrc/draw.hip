@@ -39,7 +39,7 @@ constexpr double kUnit = 8796093022208.0;  // 2^43
 constexpr int kPickThreads = 1024, kPickWaves = kPickThreads / 64;
 constexpr int kParts = kPickThreads;  // parts that a bin of many keys is split into
 constexpr int kSettle = 256;          // keys settled by comparing each with each
-constexpr int kCached = 2048;         // keys of a light row kept in LDS
+constexpr int kOrdered = 2 * kPickThreads;  // keys put in order at once
 constexpr int kMaxSlices = kDrawMaxVocab / kSliceTokens;
 
 struct DrawOptions {
@@ -81,13 +81,9 @@ __device__ __forceinline__ int bins_below(float top, float y) {
 __device__ __forceinline__ double draw_power(float x, float top, double inv_t) {
   return (static_cast<double>(x) - static_cast<double>(top)) * inv_t;
 }
-// 2^z in units of 2^-43, to the nearest whole number (z <= 0): 2^z = 2^n e^r with
-// |r| <= ln(2) / 2, e^r by its series through r^11 (the rest is below 2^-47), and
-// the rounding by an addition of 2^52, whose sum holds the number in its low bits.
-__device__ __forceinline__ unsigned long long draw_weight(float x, float top, double inv_t) {
-  if (x == top) return 1ull << kUnitBits;
-  const double z = draw_power(x, top, inv_t);
-  if (!(z > -45.0)) return 0ull;
+// 2^(z + shift) for z in [-1000, 0]: 2^z = 2^n e^r with |r| <= ln(2) / 2, e^r by
+// its series through r^11 (the rest is below 2^-47).
+__device__ __forceinline__ double draw_exp2(double z, int shift) {
   const double n = rint(z), r = (z - n) * 0.69314718055994530942;
   double e = 1.0 / 39916800.0;
   e = fma(e, r, 1.0 / 3628800.0);
@@ -101,8 +97,15 @@ __device__ __forceinline__ unsigned long long draw_weight(float x, float top, do
   e = fma(e, r, 0.5);
   e = fma(e, r, 1.0);
   e = fma(e, r, 1.0);
-  const double w = ldexp(e, static_cast<int>(n) + kUnitBits) + 4503599627370496.0;
-  return static_cast<unsigned long long>(__double_as_longlong(w)) & 0xfffffffffffffull;
+  return ldexp(e, static_cast<int>(n) + shift);
+}
+// A weight in units of 2^-43, to the nearest whole number: rounded by an
+// addition of 2^52, whose sum holds the number in its low bits.
+__device__ __forceinline__ unsigned long long draw_weight(float x, float top, double inv_t) {
+  if (x == top) return 1ull << kUnitBits;
+  const double z = draw_power(x, top, inv_t);
+  if (!(z > -45.0)) return 0ull;
+  return static_cast<unsigned long long>(__double_as_longlong(draw_exp2(z, kUnitBits) + 4503599627370496.0)) & 0xfffffffffffffull;
 }
 
 // ---------------------------------------------------------------- slices
@@ -192,13 +195,15 @@ __global__ __launch_bounds__(kSliceThreads) void draw_slices_kernel(DrawArgs a, 
 // ------------------------------------------------------------------ pick
 struct PickShared {
   float top[kMaxSlices];
-  int below[kMaxSlices];                   // bins from the row's top bin to the slice's
-  int first[kMaxSlices], end[kMaxSlices];  // the places of a bin's (or of several bins') tokens in each slice's list
-  unsigned long long mass[kBins];          // running weight through each bin
-  unsigned number[kBins];                  // running count
-  unsigned long long part_mass[kParts], cache[kCached];
+  int below[kMaxSlices];                     // bins from the row's top bin to the slice's
+  double scale[kMaxSlices];                  // the slice's largest weight
+  int first[kMaxSlices];                     // a range of bins' first place in each slice's list (-1: not listed)
+  int start[kMaxSlices + 1];                 // listed tokens of the range before each slice
+  unsigned long long mass[kBins];            // running weight through each bin
+  unsigned number[kBins], next[kBins];       // running count; the next free place
+  unsigned long long key[kOrdered], sorted[kOrdered];  // key: running weights, once sorted holds the keys
+  unsigned long long part_mass[kParts];
   unsigned part_number[kParts];
-  unsigned long long key[kSettle], weight[kSettle];
   float wave_top[kPickWaves];
   unsigned long long wave_mass[kPickWaves];
   unsigned wave_number[kPickWaves];
@@ -210,79 +215,77 @@ struct PickShared {
 enum : int { kByCount = 0, kByMass = 1, kByKey = 2 };
 
 struct Picker {
-  const DrawArgs &a;
-  const DrawScratch &w;
   PickShared &sh;
   DrawOptions o;
-  int r, slices;
+  int slices, vocab;
   float top, ytop, penalty;
   const float *logits;
   const int32_t *counts;
-  int cached = -1;  // keys in sh.cache, those of the bins through cached_bin (-1: none)
-  int cached_bin = -1;
+  const uint16_t *ends, *list;  // the row's
 
   __device__ __forceinline__ int bin_at(float x) const { return bins_below(ytop, bin_floor(x, o.bin_scale)); }
 
   // The list places of bins g0 .. g1 in every slice (then a barrier).
   __device__ __forceinline__ void places(int g0, int g1) const {
-    for (int s = threadIdx.x; s < slices; s += kPickThreads) {
-      int first = 0, end = 0;
+    const int s = threadIdx.x;
+    int first = 0, end = 0;
+    if (s < slices && sh.top[s] != -INFINITY) {
       // the slice's bins: its own bin b is the row's b + below, the last takes
-      // all that lies further down
-      const int b0 = max(g0 - sh.below[s], 0), b1 = g1 == kBins - 1 ? kBins - 1 : g1 - sh.below[s];
-      if (sh.top[s] != -INFINITY && b1 >= 0 && (g1 == kBins - 1 || g0 - sh.below[s] < kBins - 1)) {
-        const uint16_t *ends = w.ends + (static_cast<size_t>(r) * w.slices + s) * kBins;
-        // (a slice's last bin holds bins of the row beyond g1 too, so a range that
-        // ends in it, short of the row's last, takes only what lies before)
-        const int last = g1 == kBins - 1 ? kBins - 1 : min(b1, kBins - 2);
-        first = b0 > 0 ? ends[b0 - 1] : 0;
-        end = ends[last];
+      // all that lies further down (so a range that ends in it, short of the
+      // row's last, takes only what lies before)
+      const int below = sh.below[s], b0 = max(g0 - below, 0), b1 = g1 == kBins - 1 ? kBins - 1 : min(g1 - below, kBins - 2);
+      if (b1 >= b0) {
+        first = b0 > 0 ? ends[s * kBins + b0 - 1] : 0;
+        end = max(first, static_cast<int>(ends[s * kBins + b1]));
       }
-      sh.first[s] = first;
-      sh.end[s] = max(first, end);
     }
+    const bool listed = end <= kListed && !(o.light && first >= o.top_k);
+    unsigned long long unused = 0ull;
+    unsigned through = listed ? end - first : 0;
+    running(unused, through);
+    if (s < slices) {
+      sh.first[s] = listed || first == end ? first : -1;
+      sh.start[s + 1] = static_cast<int>(through);
+    }
+    if (s == 0) sh.start[0] = 0;
     __syncthreads();
   }
-  // f(key) for every key of bins g0 .. g1, from the places in sh.first / sh.end
+  // f(key) for every key of bins g0 .. g1, from what places() left
   template <typename F>
   __device__ __forceinline__ void for_each(int g0, int g1, F f) const {
-    if (cached >= 0 && g1 <= cached_bin) {
-      for (int e = threadIdx.x; e < cached; e += kPickThreads) {
-        const unsigned long long k = sh.cache[e];
-        const int bin = bin_at(argmax_key_value(k));
-        if (bin >= g0 && bin <= g1) f(k);
-      }
-      return;
+    const int listed = sh.start[slices];
+#pragma unroll 1
+    for (int i = threadIdx.x; i < listed; i += kPickThreads) {
+      int s = 0;  // the last slice that starts at or before i
+#pragma unroll
+      for (int step = kMaxSlices / 2; step > 0; step >>= 1)
+        if (s + step < slices && sh.start[s + step] <= i) s += step;
+      const int t = s * kSliceTokens + list[s * kListed + sh.first[s] + i - sh.start[s]];
+      f(argmax_key(draw_value(logits[t], counts != nullptr ? counts[t] : 0, penalty), static_cast<uint32_t>(t)));
     }
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+#pragma unroll 1
     for (int s = wave; s < slices; s += kPickWaves) {
-      const int first = sh.first[s], end = sh.end[s], t0 = s * kSliceTokens;
-      if (first >= end) continue;
-      if (end <= kListed && !(o.light && first >= o.top_k)) {
-        const uint16_t *list = w.list + (static_cast<size_t>(r) * w.slices + s) * kListed;
-        for (int e = first + lane; e < end; e += 64) {
-          const int t = t0 + list[e];
-          f(argmax_key(draw_value(logits[t], counts != nullptr ? counts[t] : 0, penalty), static_cast<uint32_t>(t)));
+      if (sh.first[s] >= 0) continue;
+      constexpr int U = 8;
+      const int t0 = s * kSliceTokens;
+#pragma unroll 1
+      for (int e = lane; e < kSliceTokens && t0 + e < vocab; e += 64 * U) {
+        float x[U];
+        int seen[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int t = min(t0 + e + 64 * u, vocab - 1);
+          x[u] = logits[t];
+          seen[u] = counts != nullptr ? counts[t] : 0;
         }
-      } else {
-        constexpr int U = 8;
-        for (int e = lane; e < kSliceTokens && t0 + e < a.vocab; e += 64 * U) {
-          float x[U];
-          int seen[U];
 #pragma unroll
-          for (int u = 0; u < U; ++u) {
-            const int t = min(t0 + e + 64 * u, a.vocab - 1);
-            x[u] = logits[t];
-            seen[u] = counts != nullptr ? counts[t] : 0;
-          }
-#pragma unroll
-          for (int u = 0; u < U; ++u) {
-            const int t = t0 + e + 64 * u;
-            const float v = draw_value(x[u], seen[u], penalty);
-            if (e + 64 * u >= kSliceTokens || t >= a.vocab || v == -INFINITY) continue;
-            const int bin = bin_at(v);
-            if (bin >= g0 && bin <= g1) f(argmax_key(v, static_cast<uint32_t>(t)));
-          }
+        for (int u = 0; u < U; ++u) {
+          const int t = t0 + e + 64 * u;
+          const float v = draw_value(x[u], seen[u], penalty);
+          if (t >= vocab || v == -INFINITY) continue;
+          const int bin = bin_at(v);
+          if (bin >= g0 && bin <= g1) f(argmax_key(v, static_cast<uint32_t>(t)));
         }
       }
     }
@@ -310,30 +313,90 @@ struct Picker {
       c += sh.wave_number[v];
     }
   }
-  // sh.mass / sh.number from each bin's own to running sums
+  // sh.mass / sh.number from each bin's own to running sums: three bins per lane
+  // of the first wavefront
   __device__ __forceinline__ void running_bins() const {
-    const int tid = threadIdx.x;
+    static_assert(kBins == 3 * 64, "three bins per lane");
+    const int lane = threadIdx.x;
     __syncthreads();
-    unsigned long long m = tid < kBins ? sh.mass[tid] : 0ull;
-    unsigned c = tid < kBins ? sh.number[tid] : 0u;
-    running(m, c);
-    if (tid < kBins) {
-      sh.mass[tid] = m;
-      sh.number[tid] = c;
+    if (lane < 64) {
+      unsigned long long m[3], run_m = 0ull;
+      unsigned c[3], run_c = 0u;
+#pragma unroll
+      for (int e = 0; e < 3; ++e) {
+        m[e] = run_m += sh.mass[3 * lane + e];
+        c[e] = run_c += sh.number[3 * lane + e];
+      }
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) {
+        const unsigned long long um = __shfl(run_m, max(lane - d, 0), 64);
+        const unsigned uc = __shfl(run_c, max(lane - d, 0), 64);
+        if (lane >= d) {
+          run_m += um;
+          run_c += uc;
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 3; ++e) {
+        sh.mass[3 * lane + e] = run_m - m[2] + m[e];
+        sh.number[3 * lane + e] = run_c - c[2] + c[e];
+      }
     }
     __syncthreads();
+  }
+
+  // The keys through bin g, all n of them (at most kOrdered), in sh.sorted, and
+  // their running weights in sh.key: bin by bin to begin with, then each key's
+  // place by comparing it with its bin's.
+  __device__ __forceinline__ void in_order(int g, int n) const {
+    const int tid = threadIdx.x;
+    if (tid < kBins) sh.next[tid] = tid > 0 ? sh.number[tid - 1] : 0u;
+    places(0, g);
+    for_each(0, g, [&](unsigned long long k) { sh.key[atomicAdd(&sh.next[bin_at(argmax_key_value(k))], 1u)] = k; });
+    __syncthreads();
+#pragma unroll 1
+    for (int i = tid; i < n; i += kPickThreads) {
+      const unsigned long long k = sh.key[i];
+      const int bin = bin_at(argmax_key_value(k)), end = static_cast<int>(sh.number[bin]);
+      int place = bin > 0 ? static_cast<int>(sh.number[bin - 1]) : 0;
+#pragma unroll 4
+      for (int e = place; e < end; ++e) place += sh.key[e] > k ? 1 : 0;
+      sh.sorted[place] = k;
+    }
+    __syncthreads();
+    static_assert(kOrdered == 2 * kPickThreads, "two keys per thread");
+    unsigned long long m = 0ull, last = 0ull;
+#pragma unroll 1
+    for (int i = 2 * tid; i < min(n, 2 * tid + 2); ++i) m += last = draw_weight(argmax_key_value(sh.sorted[i]), top, o.inv_t);
+    const bool both = 2 * tid + 1 < n;
+    unsigned unused = 0u;
+    running(m, unused);
+    if (both) sh.key[2 * tid + 1] = m;
+    if (2 * tid < n) sh.key[2 * tid] = both ? m - last : m;
+    __syncthreads();
+  }
+  // The first of places 0 .. n - 1 that satisfies f, which holds for all after one
+  // it holds for; n - 1 if none does. Every wavefront looks for itself.
+  template <typename F>
+  __device__ __forceinline__ int first_place(int n, F f) const {
+    static_assert(kOrdered == 64 * 32, "64 lanes look at every 32nd");
+    const int lane = threadIdx.x & 63;
+    int e = 32 * lane + 31;
+    const int c = 32 * __builtin_ctzll(q35_ballot(e >= n - 1 || f(min(e, n - 1))));
+    e = c + (lane & 31);
+    return c + __builtin_ctzll(q35_ballot(e >= n - 1 || f(min(e, n - 1))));
   }
 
   // The position in bin g at which the running count or weight reaches
   // `target` (kByCount, kByMass), or of the last key at or above it (kByKey):
   // sh.result_key and sh.result_mass, the running weight through it.
-  __device__ void settle(int g, int mode, unsigned long long target) const {
+  __device__ __forceinline__ void settle(int g, int mode, unsigned long long target) const {
     const int tid = threadIdx.x;
     unsigned long long before = g > 0 ? sh.mass[g - 1] : 0ull;
     unsigned above = g > 0 ? sh.number[g - 1] : 0u;
     int n = static_cast<int>(sh.number[g] - above);
     __syncthreads();  // the last settle's readers are done
-    if (!(cached >= 0 && g <= cached_bin)) places(g, g);
+    places(g, g);
     unsigned long long low = 0ull, high = ~0ull;
     if (n > kSettle && g < kBins - 1) {
       // keys of values whose x * scale may round into the bin
@@ -407,7 +470,7 @@ struct Picker {
       if (k < low || k > high) return;
       const unsigned i = atomicAdd(&sh.found, 1u);
       sh.key[i] = k;
-      sh.weight[i] = draw_weight(argmax_key_value(k), top, o.inv_t);
+      sh.sorted[i] = draw_weight(argmax_key_value(k), top, o.inv_t);
     });
     __syncthreads();
     const int i = tid >> 2, q = tid & 3;
@@ -416,7 +479,7 @@ struct Picker {
     unsigned c = 0u;
     for (int e = q; e < n; e += 4) {
       if (sh.key[e] >= mine) {
-        m += sh.weight[e];
+        m += sh.sorted[e];
         ++c;
       }
     }
@@ -425,7 +488,7 @@ struct Picker {
       m += __shfl_xor(m, d, 64);
       c += __shfl_xor(c, d, 64);
     }
-    const unsigned long long own = i < n ? sh.weight[i] : 0ull;
+    const unsigned long long own = i < n ? sh.sorted[i] : 0ull;
     // without a key that meets the condition: the last one that weighs (as above)
     if (q == 0 && i < n && mode == kByMass && own != 0ull) atomicMax(&sh.result_mass, before + m);
     __syncthreads();
@@ -453,7 +516,7 @@ struct Picker {
 
   // The first bin whose running count or weight reaches the target (the last
   // bin, where rounding leaves none).
-  __device__ int bin_of(int mode, unsigned long long target) const {
+  __device__ __forceinline__ int bin_of(int mode, unsigned long long target) const {
     const int tid = threadIdx.x;
     __syncthreads();
     if (tid == 0) sh.where = kBins - 1;
@@ -467,59 +530,114 @@ struct Picker {
     return sh.where;
   }
 
-  // A light row: the weights of the bins through g, and their keys where they
-  // are not too many (the bins beyond hold none).
-  __device__ __forceinline__ void weigh(int g) {
-    const int tid = threadIdx.x, n = static_cast<int>(sh.number[g]);
-    __syncthreads();
+  // A light row: the running weights of the bins through g (the bins beyond hold
+  // none); the counts are running already.
+  __device__ __forceinline__ void weigh(int g) const {
+    const int tid = threadIdx.x;
     if (tid < kBins) sh.mass[tid] = 0ull;
-    if (tid == 0) sh.found = 0u;
     places(0, g);
-    const bool keep = n <= kCached;
     for_each(0, g, [&](unsigned long long k) {
       const float x = argmax_key_value(k);
       const unsigned long long m = draw_weight(x, top, o.inv_t);
       if (m != 0ull) atomicAdd(&sh.mass[bin_at(x)], m);
-      if (keep) sh.cache[atomicAdd(&sh.found, 1u)] = k;
     });
     __syncthreads();
-    if (keep) {
-      cached = n;
-      cached_bin = g;
-    }
-    // running weights; the counts are running already
     unsigned long long m = tid < kBins ? sh.mass[tid] : 0ull;
-    unsigned c = 0u;
-    running(m, c);
+    unsigned unused = 0u;
+    running(m, unused);
     if (tid < kBins) sh.mass[tid] = m;
     __syncthreads();
   }
 };
 
+// The place of a drawn number in a weight of `cut`: 1 .. cut.
+__device__ __forceinline__ unsigned long long draw_target(float u, unsigned long long cut) {
+  const double at = floor((u > 0.0F ? static_cast<double>(u) : 0.0) * static_cast<double>(cut));
+  return at >= static_cast<double>(cut) ? cut : min(static_cast<unsigned long long>(at) + 1ull, cut);
+}
+__device__ __forceinline__ unsigned long long draw_nucleus(float top_p, unsigned long long kept) {
+  const double want = ceil(fmax(static_cast<double>(top_p), 0.0) * static_cast<double>(kept));
+  return want < 1.0 ? 1ull : min(static_cast<unsigned long long>(want), kept);
+}
+
+// The draw where a cut has too many keys before it to put them in order: every
+// cut is settled in its own bin. Leaves the key in sh.result_key and returns the
+// weight drawn from. (Apart from the kernel, whose instructions are all fetched
+// anew by every launch: this is the part that it seldom reaches.)
+__device__ __attribute__((noinline)) unsigned long long draw_settled(Picker p, unsigned top_k, unsigned total, float least, float u) {
+  PickShared &sh = p.sh;
+  if (p.o.light) p.weigh(p.bin_of(kByCount, top_k > 0u ? top_k : total));
+  unsigned long long kept = sh.mass[kBins - 1];
+  unsigned long long cut = kept;
+  // the first top_k, the keys from `least` on, the nucleus, the drawn one
+#pragma unroll 1
+  for (int step = 0; step < 4; ++step) {
+    int mode = kByMass, g = 0;
+    unsigned long long target = 0ull;
+    if (step == 0) {
+      if (top_k == 0u) continue;
+      mode = kByCount;
+      target = top_k;
+    } else if (step == 1) {
+      if (least == -INFINITY) continue;
+      g = p.bin_at(least);
+      if (g > 0 && sh.mass[g - 1] >= cut) continue;  // beyond the first top_k
+      mode = kByKey;
+      target = argmax_key(least, 0xffffffffu);
+    } else if (step == 2) {
+      if (p.o.top_p >= 1.0F) continue;
+      target = draw_nucleus(p.o.top_p, kept);
+      if (target >= cut) continue;
+    } else {
+      target = draw_target(u, cut);
+    }
+    if (mode != kByKey) g = p.bin_of(mode, target);
+    p.settle(g, mode, target);
+    if (step == 0) kept = cut = sh.result_mass;
+    else if (step < 3 && sh.result_mass < cut) cut = sh.result_mass;
+  }
+  return cut;
+}
+
 __global__ __launch_bounds__(kPickThreads) void draw_pick_kernel(DrawArgs a, DrawScratch w) {
   __shared__ PickShared sh;
-  const int r = static_cast<int>(blockIdx.x), tid = threadIdx.x;
+  const int r = static_cast<int>(blockIdx.x), tid = threadIdx.x, slices = w.slices;
+  const size_t row = static_cast<size_t>(r) * slices;
   const float penalty = a.penalties != nullptr ? a.penalties[r] : 1.0F;
-  Picker p{a,
-           w,
-           sh,
+  Picker p{sh,
            draw_options(a, r),
-           r,
-           w.slices,
+           slices,
+           a.vocab,
            -INFINITY,
            0.0F,
            penalty,
            a.logits + static_cast<size_t>(r) * a.stride,
-           a.counts != nullptr && penalty > 1.0F ? a.counts + static_cast<size_t>(r) * a.vocab : nullptr};
+           a.counts != nullptr && penalty > 1.0F ? a.counts + static_cast<size_t>(r) * a.vocab : nullptr,
+           w.ends + row * kBins,
+           w.list + row * kListed};
   const float u = a.uniforms[r];
+  // the slices' bins, four to a thread, U times; the first are asked for together
+  // with the slices' largest values
+  constexpr int U = 3, kFours = kBins / 4;
+  const int fours = slices * kFours;
+  q35_u32x2 ends[U];
+  unsigned last[U];
+  q35_u64x2 mass[U][2];
+  auto ask = [&](int e0) {
+#pragma unroll
+    for (int v = 0; v < U; ++v) {
+      const int at = 4 * min(e0 + v * kPickThreads, fours - 1);
+      ends[v] = *reinterpret_cast<const q35_u32x2 *>(p.ends + at);
+      last[v] = p.ends[max(at - 1, 0)];
+      if (p.o.light) continue;
+      mass[v][0] = *reinterpret_cast<const q35_u64x2 *>(w.mass + row * kBins + at);
+      mass[v][1] = *reinterpret_cast<const q35_u64x2 *>(w.mass + row * kBins + at + 2);
+    }
+  };
   // the row's largest value and each slice's distance from it
-  float top = -INFINITY;
-  for (int s = tid; s < w.slices; s += kPickThreads) {
-    const float x = w.top[static_cast<size_t>(r) * w.slices + s];
-    sh.top[s] = x;
-    top = fmaxf(top, x);
-  }
-  top = group_max<64>(top);
+  const float own = tid < slices ? w.top[row + tid] : -INFINITY;
+  ask(tid);
+  float top = group_max<64>(own);
   if ((tid & 63) == 0) sh.wave_top[tid >> 6] = top;
   if (tid < kBins) {
     sh.mass[tid] = 0ull;
@@ -537,71 +655,86 @@ __global__ __launch_bounds__(kPickThreads) void draw_pick_kernel(DrawArgs a, Dra
   }
   p.top = top;
   p.ytop = bin_floor(top, p.o.bin_scale);
-  for (int s = tid; s < w.slices; s += kPickThreads) sh.below[s] = bins_below(p.ytop, bin_floor(sh.top[s], p.o.bin_scale));
+  if (tid < slices) {
+    sh.top[tid] = own;
+    sh.below[tid] = bins_below(p.ytop, bin_floor(own, p.o.bin_scale));
+    sh.scale[tid] = own == top ? 1.0 : draw_exp2(fmax(draw_power(own, top, p.o.inv_t), -1000.0), 0);
+  }
   __syncthreads();
-  // the slices' bins, four to a thread, weights brought from each slice's
-  // largest to the row's
-  for (int e = tid; e < w.slices * (kBins / 4); e += kPickThreads) {
-    const int s = e / (kBins / 4), bin = 4 * (e - s * (kBins / 4));
-    const float x = sh.top[s];
-    if (x == -INFINITY) continue;
-    const size_t at = (static_cast<size_t>(r) * w.slices + s) * kBins + bin;
-    const q35_u32x2 ends = *reinterpret_cast<const q35_u32x2 *>(w.ends + at);
-    unsigned last = bin > 0 ? w.ends[at - 1] : 0u;
-    const double scale = x == top ? 1.0 : exp2(fmax(draw_power(x, top, p.o.inv_t), -1000.0));
+  // weights brought from each slice's largest to the row's
+#pragma unroll 1
+  for (int e0 = tid; e0 < fours; e0 += U * kPickThreads) {
+    if (e0 != tid) ask(e0);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const unsigned end = (ends[k >> 1] >> (16 * (k & 1))) & 0xffffu, n = end - last;
-      last = end;
-      if (n == 0u) continue;
-      const int g = min(kBins - 1, sh.below[s] + bin + k);
-      atomicAdd(&sh.number[g], n);
-      if (p.o.light) continue;
-      const unsigned long long m = static_cast<unsigned long long>(static_cast<double>(w.mass[at + k]) * scale + 0.5);
-      if (m != 0ull) atomicAdd(&sh.mass[g], m);
+    for (int v = 0; v < U; ++v) {
+      const int e = e0 + v * kPickThreads, s = e / kFours, bin = 4 * (e - s * kFours);
+      if (e >= fours || sh.top[s] == -INFINITY) continue;
+      unsigned before = bin > 0 ? last[v] : 0u;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const unsigned end = (ends[v][k >> 1] >> (16 * (k & 1))) & 0xffffu, n = end - before;
+        before = end;
+        if (n == 0u) continue;
+        const int g = min(kBins - 1, sh.below[s] + bin + k);
+        atomicAdd(&sh.number[g], n);
+        if (p.o.light) continue;
+        const unsigned long long own_mass = mass[v][k >> 1][k & 1];
+        const unsigned long long m = static_cast<unsigned long long>(static_cast<double>(own_mass) * sh.scale[s] + 0.5);
+        if (m != 0ull) atomicAdd(&sh.mass[g], m);
+      }
     }
   }
   p.running_bins();
   const unsigned total = sh.number[kBins - 1];
-  const int top_k = p.o.top_k > 0 && static_cast<unsigned>(p.o.top_k) < total ? p.o.top_k : 0;
-  if (p.o.light) p.weigh(p.bin_of(kByCount, top_k > 0 ? top_k : total));
-  unsigned long long kept = sh.mass[kBins - 1];
-  if (top_k > 0) {
-    p.settle(p.bin_of(kByCount, top_k), kByCount, top_k);
-    kept = sh.result_mass;
-  }
-  unsigned long long cut = kept;
+  const unsigned top_k = p.o.top_k > 0 && static_cast<unsigned>(p.o.top_k) < total ? p.o.top_k : 0u;
+  // the smallest value that weighs min_p, rounded up to fp32 (-inf: no such cut)
+  float least = -INFINITY;
   if (p.o.min_p > 0.0F && top != INFINITY) {
-    // the smallest value that weighs min_p, rounded up to fp32
-    const double least = static_cast<double>(top) + log2(fmin(static_cast<double>(p.o.min_p), 1.0)) / p.o.inv_t;
-    float x = static_cast<float>(least);
-    if (static_cast<double>(x) < least) x = nextafterf(x, INFINITY);
-    x = fminf(x, top) + 0.0F;
-    const int g = x > -INFINITY ? p.bin_at(x) : kBins - 1;
-    if (x > -INFINITY && (g == 0 || sh.mass[g - 1] < cut)) {  // (else it lies beyond the first top_k)
-      p.settle(g, kByKey, argmax_key(x, 0xffffffffu));
-      cut = sh.result_mass < cut ? sh.result_mass : cut;
-    }
+    const double x = static_cast<double>(top) + log2(fmin(static_cast<double>(p.o.min_p), 1.0)) / p.o.inv_t;
+    least = static_cast<float>(x);
+    if (static_cast<double>(least) < x) least = nextafterf(least, INFINITY);
+    least = fminf(least, top) + 0.0F;
   }
-  if (!(p.o.top_p >= 1.0F)) {
-    const double want = ceil(fmax(static_cast<double>(p.o.top_p), 0.0) * static_cast<double>(kept));
-    unsigned long long target = want < 1.0 ? 1ull : static_cast<unsigned long long>(want);
-    if (target > kept) target = kept;
-    if (target < cut) {  // (else it lies beyond the cut there is)
-      p.settle(p.bin_of(kByMass, target), kByMass, target);
-      cut = sh.result_mass < cut ? sh.result_mass : cut;
-    }
+  // The bin through which keys have to be put in order: the first top_k's, whose
+  // weight the nucleus needs, or the nearest cut's, or that of the drawn key.
+  const bool by_count = p.o.light || top_k > 0u;
+  int g = kBins - 1;
+  if (top_k > 0u) {
+    g = p.bin_of(kByCount, top_k);
+  } else if (!by_count) {
+    const unsigned long long all = sh.mass[kBins - 1];
+    if (least != -INFINITY) g = p.bin_at(least);
+    if (!(p.o.top_p >= 1.0F)) g = min(g, p.bin_of(kByMass, draw_nucleus(p.o.top_p, all)));
+    else if (least == -INFINITY) g = p.bin_of(kByMass, draw_target(u, all));
   }
-  const double at = floor((u > 0.0F ? static_cast<double>(u) : 0.0) * static_cast<double>(cut));
-  unsigned long long target = at >= static_cast<double>(cut) ? cut : static_cast<unsigned long long>(at) + 1ull;
-  if (target > cut) target = cut;
-  p.settle(p.bin_of(kByMass, target), kByMass, target);
+  const int n = static_cast<int>(sh.number[g]);
+  unsigned long long cut;
+  if (n <= kOrdered) {
+    p.in_order(g, n);
+    const unsigned long long *running = sh.key, most = running[n - 1];
+    auto place_of = [&](unsigned long long target) {
+      target = min(target, most);  // (the bins' weights, rounded once more, may pass the keys')
+      return p.first_place(n, [&](int e) { return running[e] >= target; });
+    };
+    const unsigned long long kept = top_k > 0u ? running[top_k - 1] : by_count ? most : sh.mass[kBins - 1];
+    cut = kept;
+    if (least != -INFINITY) {
+      const unsigned long long bound = argmax_key(least, 0xffffffffu);
+      const int e = p.first_place(n, [&](int i) { return sh.sorted[i] < bound; });
+      cut = min(cut, running[e > 0 && sh.sorted[e] < bound ? e - 1 : e]);
+    }
+    if (!(p.o.top_p >= 1.0F)) cut = min(cut, running[place_of(draw_nucleus(p.o.top_p, kept))]);
+    const int e = place_of(draw_target(u, cut));
+    if (tid == 0) sh.result_key = sh.sorted[e];
+  } else {
+    cut = draw_settled(p, top_k, total, least, u);
+  }
   if (tid == 0) {
     const unsigned long long key = sh.result_key;
     const float x = argmax_key_value(key);
     a.out_token[r] = static_cast<int32_t>(argmax_key_index(key));
     if (a.out_probability != nullptr)
-      a.out_probability[r] = static_cast<float>((x == top ? 1.0 : exp2(draw_power(x, top, p.o.inv_t))) * kUnit / static_cast<double>(cut));
+      a.out_probability[r] = static_cast<float>((x == top ? 1.0 : draw_exp2(fmax(draw_power(x, top, p.o.inv_t), -1000.0), 0)) * kUnit / static_cast<double>(cut));
   }
 }
 

@@ -48,6 +48,7 @@ typedef float q35_f32x16 __attribute__((ext_vector_type(16)));
 // marked non-temporal so they do not displace reused lines in L1/L2.
 typedef unsigned int q35_u32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned int q35_u32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned long long q35_u64x2 __attribute__((ext_vector_type(2)));
 typedef float q35_f32x4 __attribute__((ext_vector_type(4)));
 typedef float q35_f32x2 __attribute__((ext_vector_type(2)));
 #define Q35_LOAD_NT(ptr) __builtin_nontemporal_load(ptr)

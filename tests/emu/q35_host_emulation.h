@@ -295,6 +295,7 @@ inline q35emu_v4i q35emu_mfma_i8(long a, long b, q35emu_v4i c) {
 #define Q35_MFMA_I32_16X16X32_I8(a, b, c, cbsz, abid, blgp) q35emu_mfma_i8(a, b, c)
 typedef unsigned int q35_u32x4 __attribute__((vector_size(16)));
 typedef unsigned int q35_u32x2 __attribute__((vector_size(8)));
+typedef unsigned long long q35_u64x2 __attribute__((vector_size(16)));
 typedef float q35_f32x4 __attribute__((vector_size(16)));
 typedef float q35_f32x2 __attribute__((vector_size(8)));
 // fp16 MFMA (v_mfma_f32_16x16x32_f16): the i8 operand layout with eight
