@@ -145,11 +145,12 @@ __global__ __launch_bounds__(kSliceThreads) void draw_slices_kernel(DrawArgs a, 
   if (tid == 0) w.top[at] = top;
   if (top == -INFINITY) return;  // whole workgroup: the pick reads nothing else of such a slice
   const float ytop = bin_floor(top, o.bin_scale);
+  unsigned nth[kSlicePer];  // the token's number in its bin
 #pragma unroll
   for (int i = 0; i < kSlicePer; ++i) {
     if (x[i] == -INFINITY) continue;
     const int bin = bins_below(ytop, bin_floor(x[i], o.bin_scale));
-    atomicAdd(&number[bin], 1u);
+    nth[i] = atomicAdd(&number[bin], 1u);
     if (!o.light) {
       const unsigned long long m = draw_weight(x[i], top, o.inv_t);
       if (m != 0ull) atomicAdd(&mass[bin], m);
@@ -186,9 +187,9 @@ __global__ __launch_bounds__(kSliceThreads) void draw_slices_kernel(DrawArgs a, 
   for (int i = 0; i < kSlicePer; ++i) {
     if (x[i] == -INFINITY) continue;
     const int bin = bins_below(ytop, bin_floor(x[i], o.bin_scale));
-    if ((number[bin] & 0x80000000u) != 0u) continue;
-    const unsigned place = atomicAdd(&number[bin], 1u);
-    w.list[at * kListed + place] = static_cast<uint16_t>(tid + i * kSliceThreads);
+    const unsigned first = number[bin];
+    if ((first & 0x80000000u) != 0u) continue;
+    w.list[at * kListed + first + nth[i]] = static_cast<uint16_t>(tid + i * kSliceThreads);
   }
 }
 
