@@ -109,6 +109,8 @@ __device__ __forceinline__ unsigned long long draw_weight(float x, float top, do
 }
 
 // ---------------------------------------------------------------- slices
+typedef unsigned Four __attribute__((vector_size(16), aligned(4)));
+
 __global__ __launch_bounds__(kSliceThreads) void draw_slices_kernel(DrawArgs a, DrawScratch w) {
   __shared__ unsigned long long mass[kBins];
   __shared__ unsigned number[kBins];
@@ -121,11 +123,30 @@ __global__ __launch_bounds__(kSliceThreads) void draw_slices_kernel(DrawArgs a, 
   const DrawOptions o = draw_options(a, r);
   float x[kSlicePer];
   int seen[kSlicePer];
+  // four tokens at a time (rows need not be aligned to more than 4 bytes, which
+  // such loads take); the row's last slice token by token
+  auto token = [&](int i) { return 4 * (tid + (i >> 2) * kSliceThreads) + (i & 3); };
+  if (t0 + kSliceTokens <= a.vocab) {
 #pragma unroll
-  for (int i = 0; i < kSlicePer; ++i) {
-    const int t = min(t0 + tid + i * kSliceThreads, a.vocab - 1);
-    x[i] = logits[t];
-    seen[i] = counts != nullptr ? counts[t] : 0;
+    for (int i = 0; i < kSlicePer; i += 4) {
+      const Four v = *reinterpret_cast<const Four *>(logits + t0 + token(i));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[i + e] = __uint_as_float(v[e]);
+    }
+#pragma unroll
+    for (int i = 0; i < kSlicePer; i += 4) {
+      Four v = {0u, 0u, 0u, 0u};
+      if (counts != nullptr) v = *reinterpret_cast<const Four *>(counts + t0 + token(i));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) seen[i + e] = static_cast<int>(v[e]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kSlicePer; ++i) {
+      const int t = min(t0 + token(i), a.vocab - 1);
+      x[i] = logits[t];
+      seen[i] = counts != nullptr ? counts[t] : 0;
+    }
   }
   if (tid < kBins) {
     mass[tid] = 0ull;
@@ -134,7 +155,7 @@ __global__ __launch_bounds__(kSliceThreads) void draw_slices_kernel(DrawArgs a, 
   float top = -INFINITY;
 #pragma unroll
   for (int i = 0; i < kSlicePer; ++i) {
-    x[i] = t0 + tid + i * kSliceThreads < a.vocab ? draw_value(x[i], seen[i], penalty) : -INFINITY;
+    x[i] = t0 + token(i) < a.vocab ? draw_value(x[i], seen[i], penalty) : -INFINITY;
     top = fmaxf(top, x[i]);
   }
   top = group_max<64>(top);
@@ -189,7 +210,7 @@ __global__ __launch_bounds__(kSliceThreads) void draw_slices_kernel(DrawArgs a, 
     const int bin = bins_below(ytop, bin_floor(x[i], o.bin_scale));
     const unsigned first = number[bin];
     if ((first & 0x80000000u) != 0u) continue;
-    w.list[at * kListed + first + nth[i]] = static_cast<uint16_t>(tid + i * kSliceThreads);
+    w.list[at * kListed + first + nth[i]] = static_cast<uint16_t>(token(i));
   }
 }
 
