@@ -40,45 +40,66 @@ __global__ __launch_bounds__(kCopyThreads) void page_copy_kernel(PageCopyArgs a,
 // both is read at the step j' <= j that needs it, in the same batch of loads
 // or an earlier one. A request whose path or pages are out of bounds is left
 // as it is.
+// The first 256 rows' places in the cache are kept in LDS by the check that
+// comes before any write, so that the moves wait for three loads in all: the
+// request's path, its pages, the rows.
 constexpr int kMoveBatch = 8;
 
 template <typename T>
 __global__ __launch_bounds__(kCopyThreads) void row_compact_kernel(CompactArgs a) {
-  __shared__ int refuse;
+  __shared__ int refuse, from[kCopyThreads], to[kCopyThreads];  // rows of the pool
   const int b = static_cast<int>(blockIdx.y), tid = threadIdx.x;
   const int shift = a.page_shift, pmask = (1 << shift) - 1;
   const int capacity = a.max_pages << shift;
   const int32_t *table = a.page_table + static_cast<size_t>(b) * a.max_pages;
   const int32_t *path = a.path + static_cast<size_t>(b) * a.path_stride;
   const int context = a.context_lens[b], count = a.path_count[b];
-  if (context < 0 || context > capacity || count <= 0 || count > a.path_stride) return;  // whole workgroup
+  int p = path[min(tid, a.path_stride - 1)];
   if (tid == 0) refuse = 0;
+  if (context < 0 || context > capacity || count <= 0 || count > a.path_stride) return;  // whole workgroup
   __syncthreads();
-  auto page_ok = [&](int t) { return static_cast<unsigned>(table[t >> shift]) < static_cast<unsigned>(a.total_pages); };
-  for (int j = tid; j < count; j += kCopyThreads) {
-    const int p = path[j];
-    if (p < j || p >= capacity - context || !page_ok(context + j) || !page_ok(context + p)) refuse = 1;
+  auto place = [&](int j) {  // the rows of step j, where they are in bounds
+    const bool ok = p >= j && p < capacity - context;
+    const int t = context + j, f = context + (ok ? p : 0);
+    const int dst = ok ? table[t >> shift] : -1, src = ok ? table[f >> shift] : -1;
+    to[j & (kCopyThreads - 1)] = static_cast<int>(static_cast<unsigned>(dst) << shift) + (t & pmask);
+    from[j & (kCopyThreads - 1)] = static_cast<int>(static_cast<unsigned>(src) << shift) + (f & pmask);
+    return ok && static_cast<unsigned>(dst) < static_cast<unsigned>(a.total_pages) &&
+           static_cast<unsigned>(src) < static_cast<unsigned>(a.total_pages);
+  };
+  for (int j = (count - 1) / kCopyThreads * kCopyThreads + tid; j >= 0; j -= kCopyThreads) {  // the first 256 last
+    if (j >= count) continue;
+    if (j >= kCopyThreads || count > kCopyThreads) p = path[j];
+    if (!place(j)) refuse = 1;
   }
   __syncthreads();
   if (refuse != 0) return;
   const size_t row = static_cast<size_t>(a.row_elems) * 2 / sizeof(T);
   const size_t e = static_cast<size_t>(blockIdx.x) * kCopyThreads + tid;
   const size_t z = e / row;
-  if (z >= static_cast<size_t>(2 * a.layers)) return;
+  const bool mine = z < static_cast<size_t>(2 * a.layers);
   T *pool = reinterpret_cast<T *>((z & 1) ? a.v_pool : a.k_pool) + (z >> 1) * (a.layer_stride * 2 / sizeof(T)) + (e - z * row);
-  auto cache_row = [&](int t) { return static_cast<size_t>((table[t >> shift] << shift) + (t & pmask)) * row; };
-  for (int j0 = 0; j0 < count; j0 += kMoveBatch) {
-    T v[kMoveBatch];
-    int from[kMoveBatch];
-#pragma unroll
-    for (int u = 0; u < kMoveBatch; ++u) {
-      const int j = j0 + u;
-      from[u] = j < count ? path[j] : j;
-      if (from[u] != j) v[u] = pool[cache_row(context + from[u])];
+  for (int c = 0; c < count; c += kCopyThreads) {
+    if (c > 0) {
+      __syncthreads();
+      if (c + tid < count) {
+        p = path[c + tid];
+        place(c + tid);
+      }
+      __syncthreads();
     }
+    const int n = min(count - c, kCopyThreads);
+    for (int j0 = 0; mine && j0 < n; j0 += kMoveBatch) {
+      T v[kMoveBatch];
 #pragma unroll
-    for (int u = 0; u < kMoveBatch; ++u)
-      if (from[u] != j0 + u) pool[cache_row(context + j0 + u)] = v[u];
+      for (int u = 0; u < kMoveBatch; ++u) {
+        const int j = min(j0 + u, n - 1);
+        v[u] = pool[static_cast<size_t>(from[j]) * row];
+      }
+#pragma unroll
+      for (int u = 0; u < kMoveBatch; ++u)
+        if (j0 + u < n && from[j0 + u] != to[j0 + u]) pool[static_cast<size_t>(to[j0 + u]) * row] = v[u];
+    }
   }
 }
 

@@ -44,6 +44,7 @@ int guarded(q35_context *ctx, F body) {
 bool aligned(const void *p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
 constexpr size_t kMaxInt = static_cast<size_t>(std::numeric_limits<int32_t>::max());
+constexpr size_t kComparedPairs = 64;  // 64 x 64 comparisons take about a microsecond
 
 // The caller's workspace, or the context's own (grown as needed). A call under
 // capture needs its own: the context's may be freed by a later call that grows
@@ -281,19 +282,33 @@ extern "C" int q35_cache_copy_pages(q35_context *ctx, uint16_t *k_pool, uint16_t
     if (st != Q35_OK || count == 0) return st;
     if (src_pages == nullptr || dst_pages == nullptr)
       return set_error(ctx, Q35_ERR_INVALID, "page copy: no pages given");
-    // each page written once, and none that another pair reads: the pairs run
-    // in no order
     const int32_t pages = static_cast<int32_t>(total_pages), most = static_cast<int32_t>(page_tokens);
-    std::vector<uint8_t> written(total_pages, 0);
     for (size_t i = 0; i < count; ++i) {
       const int32_t s = src_pages[i], d = dst_pages[i];
       if (s < 0 || s >= pages || d < 0 || d >= pages || (tokens != nullptr && (tokens[i] < 0 || tokens[i] > most)))
         return set_error(ctx, Q35_ERR_INVALID, "page copy: a page outside the pool, or more tokens than a page holds");
-      if (written[d] != 0) return set_error(ctx, Q35_ERR_INVALID, "page copy: a page is written twice");
-      written[d] = 1;
     }
-    for (size_t i = 0; i < count; ++i)
-      if (written[src_pages[i]] != 0) return set_error(ctx, Q35_ERR_INVALID, "page copy: a page is both read and written");
+    // each page written once, and none that another pair reads: the pairs run
+    // in no order. Few pairs are compared with each other; more of them mark the
+    // pool's pages, which a large pool makes dear (a byte for each page).
+    bool twice = false, both = false;
+    if (count <= kComparedPairs) {
+      for (size_t i = 0; i < count; ++i) {
+        for (size_t j = 0; j < count; ++j) {
+          twice |= j < i && dst_pages[j] == dst_pages[i];
+          both |= src_pages[j] == dst_pages[i];
+        }
+      }
+    } else {
+      std::vector<uint8_t> written(total_pages, 0);
+      for (size_t i = 0; i < count; ++i) {
+        twice |= written[dst_pages[i]] != 0;
+        written[dst_pages[i]] = 1;
+      }
+      for (size_t i = 0; i < count; ++i) both |= written[src_pages[i]] != 0;
+    }
+    if (twice) return set_error(ctx, Q35_ERR_INVALID, "page copy: a page is written twice");
+    if (both) return set_error(ctx, Q35_ERR_INVALID, "page copy: a page is both read and written");
     PageCopyArgs a;
     a.k_pool = k_pool;
     a.v_pool = v_pool;

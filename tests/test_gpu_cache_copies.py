@@ -100,6 +100,26 @@ def test_copy_refusals(q, ctx):
     np.testing.assert_array_equal(dv.download(), v)
 
 
+@pytest.mark.parametrize("pairs", [63, 64, 65, 300])
+def test_copy_refusals_among_many_pairs(q, ctx, pairs):
+    rng = np.random.default_rng(pairs)
+    pages = 2 * pairs + 3
+    k, v = _pools(rng, 1, pages, 2, 8)
+    dk, dv = ctx.array(k), ctx.array(v)
+    ids = rng.permutation(pages)
+    for first, last in [(0, pairs - 1), (pairs - 2, 1)]:
+        src, dst = ids[:pairs].copy(), ids[pairs:2 * pairs].copy()
+        dst[first] = dst[last]
+        with pytest.raises(q.Q35Error, match="written twice"):
+            q.cache_copy_pages(ctx, dk, dv, 1, 0, pages, 2, 8, src, dst)
+        src, dst = ids[:pairs].copy(), ids[pairs:2 * pairs].copy()
+        src[first] = dst[last]
+        with pytest.raises(q.Q35Error, match="both read"):
+            q.cache_copy_pages(ctx, dk, dv, 1, 0, pages, 2, 8, src, dst)
+    np.testing.assert_array_equal(dk.download(), k)
+    np.testing.assert_array_equal(dv.download(), v)
+
+
 def _compact(pool, table, contexts, path, count, page_tokens):
     for b in range(len(contexts)):
         for j in range(int(count[b])):
@@ -124,6 +144,29 @@ def test_compact_rows(q, ctx, layers, page_tokens, width):
                          ctx.array(contexts), ctx.array(path), 12, ctx.array(count), 6)
     for pool, got in ((k, dk.download()), (v, dv.download())):
         _compact(_layers(pool, pages, page_tokens, width), table, contexts, path, count, page_tokens)
+        np.testing.assert_array_equal(got, pool)
+
+
+@pytest.mark.parametrize("count", [255, 256, 257, 512, 600])
+@pytest.mark.parametrize("bad", [None, 0, 254, -1])
+def test_compact_long_paths(q, ctx, count, bad):
+    """Paths of more steps than a workgroup has threads, and one bad step among
+    them, which leaves its request as it is."""
+    rng = np.random.default_rng(count)
+    page_tokens, context = 16, 21
+    path = np.arange(count, dtype=np.int32) + np.sort(rng.integers(0, 40, size=count)).astype(np.int32)
+    paths = np.stack([path, path])
+    contexts = np.full(2, context, np.int32)
+    table, pages = page_table(rng, np.full(2, context + count + 40), page_tokens)
+    k, v = _pools(rng, 1, pages, page_tokens, 24)
+    dk, dv = ctx.array(k), ctx.array(v)
+    if bad is not None:
+        paths[1, bad] = table.shape[1] * page_tokens - context  # the first row past the table
+    q.cache_compact_rows(ctx, dk, dv, 1, k.shape[1], pages, page_tokens, 24, ctx.array(table), table.shape[1],
+                         ctx.array(contexts), ctx.array(paths), count, ctx.array(np.full(2, count, np.int32)), 2)
+    moved = np.array([count, count if bad is None else 0])
+    for pool, got in ((k, dk.download()), (v, dv.download())):
+        _compact(_layers(pool, pages, page_tokens, 24), table, contexts, paths, moved, page_tokens)
         np.testing.assert_array_equal(got, pool)
 
 
