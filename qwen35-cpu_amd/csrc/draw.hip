@@ -715,7 +715,8 @@ __global__ __launch_bounds__(kPickThreads) void draw_pick_kernel(DrawArgs a, Dra
     const double x = static_cast<double>(top) + log2(fmin(static_cast<double>(p.o.min_p), 1.0)) / p.o.inv_t;
     least = static_cast<float>(x);
     if (static_cast<double>(least) < x) least = nextafterf(least, INFINITY);
-    least = fminf(least, top) + 0.0F;
+    // (at an infinite temperature every weight is 1)
+    least = p.o.inv_t > 0.0 ? fminf(least, top) + 0.0F : -INFINITY;
   }
   // The bin through which keys have to be put in order: the first top_k's, whose
   // weight the nucleus needs, or the nearest cut's, or that of the drawn key.

@@ -109,6 +109,27 @@ def test_equal_logits(q, ctx):
     _check(q, ctx, x, u, min_p=1.0, temperature=0.3)
 
 
+@pytest.mark.parametrize("options", [dict(), dict(min_p=1.0), dict(min_p=0.3, top_p=0.5), dict(top_k=7), dict(top_k=600, min_p=1.0)])
+def test_infinite_temperature(q, ctx, options):
+    """Every weight is 1, whatever the logits."""
+    x = _logits(np.random.default_rng(17), 3, 5000)
+    _check(q, ctx, x, np.array([0.0, 0.3, 0.999], np.float32), temperature=np.inf, **options)
+
+
+# around the number of keys that a row's cuts are found among at once (2048):
+# n tokens close to the largest (some equal), all others far below
+@pytest.mark.parametrize("n", [1023, 1024, 1025, 2047, 2048, 2049, 2600])
+@pytest.mark.parametrize("options", [dict(top_k=400), dict(top_k=512, top_p=0.6), dict(top_k=513, min_p=0.99, top_p=0.9),
+                                     dict(min_p=0.95), dict(top_p=0.97), dict(top_p=0.8, min_p=0.9), dict()])
+def test_many_keys_before_a_cut(q, ctx, n, options):
+    rng = np.random.default_rng(n)
+    x = (rng.standard_normal((2, 9001)) - 40).astype(np.float32)
+    for r in range(2):
+        near = np.round(rng.uniform(5.0, 5.1, size=n) * 4096) / 4096
+        x[r, rng.choice(9001, size=n, replace=False)] = near.astype(np.float32)
+    _check(q, ctx, x, np.array([0.37, 0.93], np.float32), **options)
+
+
 def test_ties_take_the_lower_token(q, ctx):
     x = np.zeros((4, 4200), np.float32)
     x[:, [4100, 17, 2000]] = 3.0
