@@ -179,7 +179,8 @@ int q35_attention_decode_paged(q35_context *ctx, const float *q, const float *ga
  * ignored): output = softmax(scale q.k) v over those rows, times
  * sigmoid(gate); a node that sees nothing, or whose scores are all -inf, gets
  * zero. Infinite or NaN keys and values reach only the nodes that see their
- * row (a key that is not finite may leave NaN in those).
+ * row (a key, or a context row's value, that is not finite may leave NaN in
+ * those).
  *   head_dim 64, 128 or 256; heads a multiple of kv_heads; page_tokens a power
  *   of two; at most 256 nodes a request; FP16 pools of total_pages pages;
  *   16-byte aligned buffers; pools, table and masks are not written.
@@ -228,7 +229,7 @@ int q35_tree_accept(q35_context *ctx, const int32_t *node_start, const int32_t *
  *     or NaN takes the first token with probability 1;
  *   top_k (0 or less, or all: off), top_p (>= 1: off; the shortest prefix that
  *     holds top_p of the weight the first top_k tokens have), min_p (<= 0:
- *     off; weights of at least min_p) each keep a prefix of the order, and the
+ *     off; weights of at least min(min_p, 1)) each keep a prefix of the order, and the
  *     shortest counts; the first token is always kept;
  *   draw: the first token at which the running weight exceeds uniforms[row]
  *     (0 <= u < 1) times the kept weight.
@@ -253,8 +254,8 @@ int q35_sample_logits(q35_context *ctx, const float *logits, size_t stride, cons
  * dst_pages[i] in every layer (tokens NULL: whole pages), KvPagesF16's copy on
  * write (include/qwen35x/cpu/kv_pages.h:52-60) for many pages at once. The
  * three arrays are HOST memory; a page written twice, or both read and
- * written, is refused, as is one outside the pool. Under stream capture the
- * pages become part of the graph. */
+ * written, is refused, as is one outside the pool. Pages have at most 2^25
+ * values. Under stream capture the pages become part of the graph. */
 int q35_cache_copy_pages(q35_context *ctx, uint16_t *k_pool, uint16_t *v_pool, size_t layers,
                          size_t layer_stride, size_t total_pages, size_t page_tokens,
                          size_t row_elems, const int32_t *src_pages, const int32_t *dst_pages,

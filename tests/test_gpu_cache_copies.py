@@ -90,7 +90,8 @@ def test_copy_refusals(q, ctx):
         with pytest.raises(q.Q35Error, match=what):
             call(*args)
     for kw, what in [(dict(layers=0), "empty"), (dict(pages=0), "empty"), (dict(page_tokens=0), "empty"), (dict(width=0), "empty"),
-                     (dict(stride=8 * 4 * 16 - 1), "overlap"), (dict(pages=2 ** 31), "2\\^31")]:
+                     (dict(stride=8 * 4 * 16 - 1), "overlap"), (dict(pages=2 ** 31), "2\\^31"),
+                     (dict(pages=2, page_tokens=2 ** 13, width=2 ** 12 + 1), "2\\^25")]:
         with pytest.raises(q.Q35Error, match=what):
             call([0], [1], **kw)
     with pytest.raises(ValueError):
