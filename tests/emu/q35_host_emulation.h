@@ -365,37 +365,6 @@ inline q35_f32x4 q35emu_mfma_f16(q35_f16x8 a, q35_f16x8 b, q35_f32x4 c) {
 }
 #define Q35_MFMA_F32_16X16X32_F16(a, b, c) q35emu_mfma_f16(a, b, c)
 typedef float q35_f32x16 __attribute__((vector_size(64)));
-// v_mfma_f32_32x32x16_f16: A lane l = row l%32, k 8*(l/32)..+7; B lane l =
-// column l%32, same k; D lane l = rows 8*(v/4) + 4*(l/32) + v%4 of column l%32
-inline q35_f32x16 q35emu_mfma_f16_32(q35_f16x8 a, q35_f16x8 b, q35_f32x16 c) {
-  auto &ctx = ::q35emu::t_ctx;
-  auto &a0 = ctx.launch->slots_a[ctx.wave], &a1 = ctx.launch->slots_b[ctx.wave];
-  auto &b0 = ctx.launch->slots_c[ctx.wave], &b1 = ctx.launch->slots_d[ctx.wave];
-  uint64_t w[4];
-  std::memcpy(w, &a, 16);
-  a0[ctx.lane] = w[0];
-  a1[ctx.lane] = w[1];
-  std::memcpy(w, &b, 16);
-  b0[ctx.lane] = w[0];
-  b1[ctx.lane] = w[1];
-  ::q35emu::wave_sync();
-  auto elem = [](const std::vector<uint64_t> &lo, const std::vector<uint64_t> &hi, int lane, int k) {
-    const uint64_t word = k < 4 ? lo[lane] : hi[lane];
-    return ::q35emu::h2f(static_cast<uint16_t>(word >> (16 * (k % 4))));
-  };
-  q35_f32x16 d;
-  const int col = ctx.lane % 32;
-  for (int v = 0; v < 16; ++v) {
-    const int row = 8 * (v / 4) + 4 * (ctx.lane / 32) + v % 4;
-    float sum = c[v];
-    for (int k = 0; k < 16; ++k)
-      sum += elem(a0, a1, row + 32 * (k / 8), k % 8) * elem(b0, b1, col + 32 * (k / 8), k % 8);
-    d[v] = sum;
-  }
-  ::q35emu::wave_sync();
-  return d;
-}
-#define Q35_MFMA_F32_32X32X16_F16(a, b, c) q35emu_mfma_f16_32(a, b, c)
 inline q35_f32x16 q35emu_mfma_outer4(float a, float b, q35_f32x16 c) {
   auto &ctx = ::q35emu::t_ctx;
   auto &as = ctx.launch->slots_a[ctx.wave], &bs = ctx.launch->slots_b[ctx.wave];
