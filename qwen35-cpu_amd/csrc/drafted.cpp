@@ -93,8 +93,9 @@ int tree_check(q35_context *ctx, size_t batch, size_t rows, size_t max_nodes, si
   a->heads = heads;
   a->kv_heads = kv_heads;
   a->head_dim = head_dim;
-  if (tree_request_units(a->max_nodes, a->max_len, heads, kv_heads) > static_cast<long long>(kMaxInt))
-    return set_error(ctx, Q35_ERR_UNSUPPORTED, "tree attention: max_len times the KV heads is too large");
+  const long long units = tree_request_units(a->max_nodes, a->max_len, heads, kv_heads);
+  if (units > static_cast<long long>(kMaxInt) || units * a->batch > kMaxTreeUnits)
+    return set_error(ctx, Q35_ERR_UNSUPPORTED, "tree attention: max_len times the KV heads and requests is too large");
   a->groups = tree_groups(a->batch, a->max_nodes, a->max_len, heads, kv_heads, ctx->cu_count);
   return Q35_OK;
 }

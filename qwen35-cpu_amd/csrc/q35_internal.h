@@ -487,7 +487,10 @@ struct TreeArgs {
   int32_t *specials = nullptr;                   // two per workgroup: node values that are not finite in a part
   float *part_o = nullptr, *part_ml = nullptr;   // two parts per workgroup: [..][head_dim], [..][2] (max, sum)
 };
-long long tree_request_units(int max_nodes, int max_len, int heads, int kv_heads);  // at most: below 2^31 for a launch
+// Work units of a request at most: below 2^31 for a launch, and all requests' at
+// most kMaxTreeUnits, so that units times workgroups are exact in fp64.
+constexpr long long kMaxTreeUnits = 1LL << 43;
+long long tree_request_units(int max_nodes, int max_len, int heads, int kv_heads);
 int tree_groups(int batch, int max_nodes, int max_len, int heads, int kv_heads, int cu_count);
 // Workspace bytes, and where specials, part_o and part_ml lie in it (first_units at 0).
 size_t tree_workspace_bytes(const TreeArgs &a, size_t *specials, size_t *part_o, size_t *part_ml);

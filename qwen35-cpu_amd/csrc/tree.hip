@@ -122,8 +122,10 @@ __device__ __forceinline__ long long tree_units(const TreeArgs &a, int b) {
 __device__ __forceinline__ int unit_groups(const TreeArgs &a, long long total) {
   return total < a.groups ? static_cast<int>(max(total, 1LL)) : a.groups;
 }
-// (Quotients of whole numbers below 2^44 by whole numbers below 2^31 or 2^9: in
-// fp64 they round to no wrong floor, and take a tenth of the integer code.)
+// (Quotients of whole numbers below 2^52, as kMaxTreeUnits and at most 512
+// workgroups leave them: in fp64 they round to no wrong floor -- a quotient short
+// of a whole number is short by more than half a step -- and take a tenth of the
+// integer code.)
 __device__ __forceinline__ long long unit_begin(int w, long long total, int groups) {
   return static_cast<long long>(floor(static_cast<double>(w * total) / groups));
 }
@@ -648,7 +650,7 @@ hipError_t launch_tree_attention(const TreeArgs &a, hipStream_t stream) {
 // Workgroups of a launch: one per CU, but not more than the units that the
 // bounds allow.
 int tree_groups(int batch, int max_nodes, int max_len, int heads, int kv_heads, int cu_count) {
-  return static_cast<int>(std::max(1LL, std::min<long long>(tree_request_units(max_nodes, max_len, heads, kv_heads) * batch, cu_count)));
+  return static_cast<int>(std::max(1LL, std::min<long long>(tree_request_units(max_nodes, max_len, heads, kv_heads) * batch, std::min(cu_count, 512))));
 }
 long long tree_request_units(int max_nodes, int max_len, int heads, int kv_heads) {
   const long long blocks = (static_cast<long long>(max_nodes) * (heads / kv_heads) + kBlockVectors - 1) / kBlockVectors;

@@ -223,3 +223,11 @@ def test_refusals(q, ctx):
         case.call(q, ctx, d)
     case.call(q, ctx, case.device(ctx), rows=0)  # no rows: nothing to do
     ctx.synchronize()
+
+
+def test_sizes_past_the_work_units(q, ctx):
+    """Bounds whose workgroup shares would no longer be exact."""
+    assert q.attention_tree_workspace(ctx, 65535, 65535, 1, 2 ** 31 - 2000, 2, 2, 64) > 0
+    for batch, heads in [(65535, 8), (1, 65)]:
+        with pytest.raises(q.Q35Error, match="too large"):
+            q.attention_tree_workspace(ctx, batch, 65535, 1, 2 ** 31 - 2000, heads, heads, 64)
