@@ -506,8 +506,10 @@ def cache_copy_pages(ctx, k_pool, v_pool, layers, layer_stride, total_pages, pag
     tokens = _page_list(tokens) if tokens is not None else None
     if src.ndim != 1 or src.shape != dst.shape or (tokens is not None and tokens.shape != src.shape):
         raise ValueError("cache_copy_pages: src, dst and tokens are lists of one length")
+    # (read before the call returns; an array's address takes numpy longer than a copy of a few pages' numbers)
     ctx.check(lib.q35_cache_copy_pages(ctx.handle, k_pool.ptr, v_pool.ptr, layers, layer_stride, total_pages, page_tokens,
-                                       row_elems, _ptr(src), _ptr(dst), _ptr(tokens), src.size), "cache_copy_pages")
+                                       row_elems, src.tobytes(), dst.tobytes(),
+                                       tokens.tobytes() if tokens is not None else None, src.size), "cache_copy_pages")
 
 
 def cache_compact_rows(ctx, k_pool, v_pool, layers, layer_stride, total_pages, page_tokens, row_elems, page_table,
