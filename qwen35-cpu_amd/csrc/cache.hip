@@ -16,8 +16,8 @@ constexpr int kCopyPieces = 4;  // pieces in flight per thread
 // One workgroup per (1024 pieces of a page, pool and layer, pair). The pairs
 // travel in the kernel's arguments, so a call stages nothing on the device. T
 // is the widest piece that the rows and the pools allow.
-template <typename T>
-__global__ __launch_bounds__(kCopyThreads) void page_copy_kernel(PageCopyArgs a, PagePairs pairs) {
+template <typename T, int N>
+__global__ __launch_bounds__(kCopyThreads) void page_copy_kernel(PageCopyArgs a, PagePairsOf<N> pairs) {
   const int i = static_cast<int>(blockIdx.x), z = static_cast<int>(blockIdx.z);
   const size_t row = static_cast<size_t>(a.row_elems) * 2 / sizeof(T);  // pieces
   const size_t n = row * pairs.tokens[i], page = row * a.page_tokens;
@@ -115,6 +115,17 @@ int piece_bytes(const void *k, const void *v, size_t row_elems, size_t layer_str
 
 }  // namespace
 
+namespace {
+template <int N>
+void launch_pairs(const PageCopyArgs &a, const PagePairsOf<N> &pairs, int piece, dim3 grid, hipStream_t stream) {
+  switch (piece) {
+    case 16: Q35_LAUNCH((page_copy_kernel<q35_u32x4, N>), grid, dim3(kCopyThreads), 0, stream, a, pairs); break;
+    case 4: Q35_LAUNCH((page_copy_kernel<uint32_t, N>), grid, dim3(kCopyThreads), 0, stream, a, pairs); break;
+    default: Q35_LAUNCH((page_copy_kernel<uint16_t, N>), grid, dim3(kCopyThreads), 0, stream, a, pairs); break;
+  }
+}
+}  // namespace
+
 hipError_t launch_page_copy(const PageCopyArgs &a, const PagePairs &pairs, int count, hipStream_t stream) {
   const int piece = piece_bytes(a.k_pool, a.v_pool, a.row_elems, a.layer_stride);
   int most = 0;  // rows of the fullest page
@@ -122,10 +133,14 @@ hipError_t launch_page_copy(const PageCopyArgs &a, const PagePairs &pairs, int c
   if (most == 0) return hipSuccess;
   const size_t pieces = static_cast<size_t>(a.row_elems) * 2 / piece * most, per = kCopyThreads * kCopyPieces;
   const dim3 grid(count, static_cast<unsigned>((pieces + per - 1) / per), 2 * a.layers);
-  switch (piece) {
-    case 16: Q35_LAUNCH((page_copy_kernel<q35_u32x4>), grid, dim3(kCopyThreads), 0, stream, a, pairs); break;
-    case 4: Q35_LAUNCH((page_copy_kernel<uint32_t>), grid, dim3(kCopyThreads), 0, stream, a, pairs); break;
-    default: Q35_LAUNCH((page_copy_kernel<uint16_t>), grid, dim3(kCopyThreads), 0, stream, a, pairs); break;
+  if (count > kFewCopyPairs) {
+    launch_pairs(a, pairs, piece, grid, stream);
+  } else {
+    PagePairsOf<kFewCopyPairs> few = {};
+    std::copy_n(pairs.src, count, few.src);
+    std::copy_n(pairs.dst, count, few.dst);
+    std::copy_n(pairs.tokens, count, few.tokens);
+    launch_pairs(a, few, piece, grid, stream);
   }
   return hipGetLastError();
 }
