@@ -168,13 +168,13 @@ __device__ void tree_row_by_row(const TreeArgs &a, const TreeRequest &rq, int i,
 
 // One workgroup of eight wavefronts. A stage's K and V rows go straight from
 // the cache to LDS (16 bytes a lane, one stage ahead of the products), each
-// read once for up to 128 vectors. With five to eight groups of 16 vectors each
-// wavefront has one and takes both tiles of a stage; with fewer, two wavefronts
-// share a group, a tile each, and are joined at the end. A wavefront keeps its
-// queries and its output in registers throughout, two wavefronts to a SIMD, so
-// that one's softmax runs beside the other's products. (Groups of 32 vectors
-// would read LDS half as often, but one wavefront then fills a SIMD's registers
-// and nothing runs beside it.)
+// read once for up to 128 vectors. Each wavefront has a group of 16 vectors and
+// takes both tiles of a stage; it keeps its queries and its output in registers
+// throughout, two wavefronts to a SIMD, so that one's softmax runs beside the
+// other's products. (Groups of 32 vectors would read LDS half as often, but one
+// wavefront then fills a SIMD's registers and nothing runs beside it. Where an
+// item has at most four groups, two wavefronts to a group, a tile each, were
+// slower: 316 against 302 us for 64 requests of up to 8192 rows and 23 nodes.)
 //
 // In LDS a K row's 16-byte pieces are rotated by xor with the row number, and a
 // V row's pairs of pieces, so that the lanes of an operand (16 rows' piece, or
@@ -194,7 +194,7 @@ __global__ __launch_bounds__(64 * kTreeWaves) Q35_WAVES_PER_EU(2) void tree_atte
   __shared__ struct __align__(1024) {
     uint16_t cache[4 * BLOCK];       // [stage % 2][K, V][row][dim]
     int rows[2 * kRowStages][kStageTokens];  // cache rows of two runs of stages (-1: none)
-    float stat[kTreeWaves][2][kGroupVectors];
+    float sums[kTreeWaves][kGroupVectors];
     long long units[kTreeWaves];
     long long first_unit;
     int first_request, special;
@@ -260,10 +260,8 @@ __global__ __launch_bounds__(64 * kTreeWaves) Q35_WAVES_PER_EU(2) void tree_atte
     const int g = item / blocks, m0 = (item - g * blocks) * kBlockVectors;
 
     const int vectors = rq.nodes * qpk, groups = min(kTreeWaves, (vectors - m0 + kGroupVectors - 1) / kGroupVectors);
-    const bool shared = groups <= kTreeWaves / 2;  // two wavefronts to a group of vectors
-    const int group = shared ? wave & (kTreeWaves / 2 - 1) : wave, part = shared ? wave / (kTreeWaves / 2) : 0;
-    const bool active = group < groups;
-    const int mg = m0 + kGroupVectors * group;
+    const bool active = wave < groups;
+    const int mg = m0 + kGroupVectors * wave;
 
     // the lane's query vector (spare lanes repeat the last one and store nothing),
     // asked for before the pages are waited for
@@ -442,50 +440,29 @@ __global__ __launch_bounds__(64 * kTreeWaves) Q35_WAVES_PER_EU(2) void tree_atte
         if (special) sh.special = 1;
       }
       if (active) {
-        for (int k = shared ? part : 0; k < (shared ? part + 1 : 2); ++k)
+        for (int k = 0; k < 2; ++k)
           if (t + kTileTokens * k < rq.len)
             tile((s & 1) * 2 * BLOCK + kTileTokens * k * HD, stage_rows(s) + kTileTokens * k, t + kTileTokens * k);
       }
     }
     lds_barrier();  // every wavefront is done with the last stage
 
-    // Each group's vectors through LDS, [vector][dims] with the 16-byte pieces
-    // of a row at their number xor the vector: first, of a shared group, the
-    // second wavefront's part, then the group's result, whose rows then leave
-    // whole, dealt over the wavefronts.
+    // Each group's vectors through LDS, [vector][dims] with the 16-byte pieces of
+    // a row at their number xor the vector, whose rows then leave whole, dealt
+    // over the wavefronts.
     sum += __shfl_xor(sum, 16, 64);
     sum += __shfl_xor(sum, 32, 64);
     constexpr int F = HD / 4;
-    q35_f32x4 *result = reinterpret_cast<q35_f32x4 *>(cache) + static_cast<size_t>(group) * (kGroupVectors * F) + col * F;
-    if (shared && active && part == 1) {
-      sh.stat[wave][0][col] = ref;
-      sh.stat[wave][1][col] = sum;
-#pragma unroll
-      for (int n = 0; n < NV; ++n) result[(4 * n + quad) ^ col] = acc[n];
-    }
-    if (shared) lds_barrier();
     const bool whole = s0 == 0 && s1 == stages;
     const size_t place = (2 * static_cast<size_t>(w) + (s0 == 0 ? 1 : 0)) * kBlockVectors;
-    if (active && part == 0) {
-      if (shared) {
-        const float *other = &sh.stat[wave + kTreeWaves / 2][0][0];
-        const float ref1 = other[col], next = fmaxf(ref, ref1), least = next == -INFINITY ? 0.0F : next;
-        const float w0 = Q35_EXP2(ref - least), w1 = Q35_EXP2(ref1 - least);
-        ref = next;
-        sum = fmaf(sum, w0, other[kGroupVectors + col] * w1);
-#pragma unroll
-        for (int n = 0; n < NV; ++n) {
-          const q35_f32x4 o = result[(4 * n + quad) ^ col];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) acc[n][i] = fmaf(o[i], w1, acc[n][i] * w0);
-        }
-      }
+    if (active) {
+      q35_f32x4 *result = reinterpret_cast<q35_f32x4 *>(cache) + static_cast<size_t>(wave) * (kGroupVectors * F) + col * F;
 #pragma unroll
       for (int n = 0; n < NV; ++n) result[(4 * n + quad) ^ col] = acc[n];
-      sh.stat[group][1][col] = sum;
+      sh.sums[wave][col] = sum;
       if (!whole && quad == 0) {
-        a.part_ml[2 * (place + kGroupVectors * group + col)] = ref;
-        a.part_ml[2 * (place + kGroupVectors * group + col) + 1] = sum;
+        a.part_ml[2 * (place + kGroupVectors * wave + col)] = ref;
+        a.part_ml[2 * (place + kGroupVectors * wave + col) + 1] = sum;
       }
     }
     lds_barrier();
@@ -503,7 +480,7 @@ __global__ __launch_bounds__(64 * kTreeWaves) Q35_WAVES_PER_EU(2) void tree_atte
         if (whole) {
           const int vn = (m0 + v) / qpk, vu = m0 + v - vn * qpk;
           const size_t to = (static_cast<size_t>(rq.row0 + vn) * a.heads + g * qpk + vu) * HD + 4 * f;
-          tree_store(a.out + to, y, sh.stat[v / kGroupVectors][1][v & (kGroupVectors - 1)], a.gates != nullptr, tree_gate(a.gates, to));
+          tree_store(a.out + to, y, sh.sums[v / kGroupVectors][v & (kGroupVectors - 1)], a.gates != nullptr, tree_gate(a.gates, to));
         } else {
           *reinterpret_cast<q35_f32x4 *>(a.part_o + (place + v) * HD + 4 * f) = y;
         }

@@ -101,7 +101,7 @@ def test_copy_refusals(q, ctx):
     np.testing.assert_array_equal(dv.download(), v)
 
 
-@pytest.mark.parametrize("pairs", [63, 64, 65, 300])
+@pytest.mark.parametrize("pairs", [16, 17, 31, 32, 33, 63, 64, 65, 300])
 def test_copy_refusals_among_many_pairs(q, ctx, pairs):
     rng = np.random.default_rng(pairs)
     pages = 2 * pairs + 3
