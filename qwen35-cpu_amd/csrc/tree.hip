@@ -509,10 +509,11 @@ __global__ __launch_bounds__(64 * kTreeWaves) Q35_WAVES_PER_EU(2) void tree_atte
   }
 }
 
-// One wavefront per (node, head), 5 us at least (its chain of loads), 15 where
-// parts, gates and output are 50 MB (64 ragged requests): the parts of its item, weights exp(m_w - M),
+// One wavefront per (node, head): the parts of its item, weights exp(m_w - M),
 // in workgroup order (the workgroups follow from the unit counts). Requests
 // that are refused on the device get NaN in their rows, where those are known.
+// 5 us at least, its chain of loads; 15 for 64 ragged requests, whose parts,
+// gates and outputs are 50 MB (four wavefronts to a workgroup: no change).
 template <int HD>
 __global__ __launch_bounds__(64) void tree_merge_kernel(TreeArgs a) {
   constexpr int F = HD / 4;  // lanes past the dims repeat them
