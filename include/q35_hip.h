@@ -254,8 +254,8 @@ int q35_sample_logits(q35_context *ctx, const float *logits, size_t stride, cons
  * dst_pages[i] in every layer (tokens NULL: whole pages), KvPagesF16's copy on
  * write (include/qwen35x/cpu/kv_pages.h:52-60) for many pages at once. The
  * three arrays are HOST memory; a page written twice, or both read and
- * written, is refused, as is one outside the pool. Pages have at most 2^25
- * values. Under stream capture the pages become part of the graph. */
+ * written, is refused, as is one outside the pool. Under stream capture the
+ * pages become part of the graph. */
 int q35_cache_copy_pages(q35_context *ctx, uint16_t *k_pool, uint16_t *v_pool, size_t layers,
                          size_t layer_stride, size_t total_pages, size_t page_tokens,
                          size_t row_elems, const int32_t *src_pages, const int32_t *dst_pages,

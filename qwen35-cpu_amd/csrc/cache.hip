@@ -28,14 +28,16 @@ __global__ __launch_bounds__(kCopyThreads) void page_copy_kernel(PageCopyArgs a,
   T *pool = reinterpret_cast<T *>((z & 1) ? a.v_pool : a.k_pool) + static_cast<size_t>(z >> 1) * (a.layer_stride * 2 / sizeof(T));
   const T *src = pool + page * pairs.src[i];
   T *dst = pool + page * pairs.dst[i];
-  const size_t at = static_cast<size_t>(blockIdx.y) * (kCopyThreads * kCopyPieces) + threadIdx.x;
-  T v[kCopyPieces];
+  for (size_t at = static_cast<size_t>(blockIdx.y) * (kCopyThreads * kCopyPieces) + threadIdx.x; at < n;
+       at += static_cast<size_t>(gridDim.y) * (kCopyThreads * kCopyPieces)) {
+    T v[kCopyPieces];
 #pragma unroll
-  for (int u = 0; u < kCopyPieces; ++u)
-    if (at + u * kCopyThreads < n) v[u] = src[at + u * kCopyThreads];
+    for (int u = 0; u < kCopyPieces; ++u)
+      if (at + u * kCopyThreads < n) v[u] = src[at + u * kCopyThreads];
 #pragma unroll
-  for (int u = 0; u < kCopyPieces; ++u)
-    if (at + u * kCopyThreads < n) dst[at + u * kCopyThreads] = v[u];
+    for (int u = 0; u < kCopyPieces; ++u)
+      if (at + u * kCopyThreads < n) dst[at + u * kCopyThreads] = v[u];
+  }
 }
 
 // Row context + path[j] of a request to row context + j, in every layer, for
@@ -136,7 +138,7 @@ hipError_t launch_page_copy(const PageCopyArgs &a, const PagePairs &pairs, int c
   for (int i = 0; i < count; ++i) most = std::max(most, pairs.tokens[i]);
   if (most == 0) return hipSuccess;
   const size_t pieces = static_cast<size_t>(a.row_elems) * 2 / piece * most, per = kCopyThreads * kCopyPieces;
-  const dim3 grid(count, static_cast<unsigned>((pieces + per - 1) / per), 2 * a.layers);
+  const dim3 grid(count, static_cast<unsigned>(std::min<size_t>((pieces + per - 1) / per, 65535)), 2 * a.layers);
   if (count > kFewCopyPairs) {
     launch_pairs(a, pairs, piece, grid, stream);
   } else {

@@ -44,7 +44,6 @@ int guarded(q35_context *ctx, F body) {
 bool aligned(const void *p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
 constexpr size_t kMaxInt = static_cast<size_t>(std::numeric_limits<int32_t>::max());
-constexpr size_t kMaxPageElems = size_t{1} << 25;
 // Up to 32 page pairs are compared with each other (0.8 us); a byte for every page
 // takes 0.1 us for 4096 pages and 25 us for a million.
 constexpr size_t kComparedPairs = 32;
@@ -117,9 +116,6 @@ int pool_check(q35_context *ctx, const void *k, const void *v, size_t layers, si
     return set_error(ctx, Q35_ERR_INVALID, "cache copy: a missing pool or an empty shape");
   if (layers > 32767 || page_tokens > (1u << 20) || row_elems > (1u << 20) || total_pages > kMaxInt / page_tokens)
     return set_error(ctx, Q35_ERR_UNSUPPORTED, "cache copy: at most 2^31 - 1 cache rows of 2^20 values");
-  // (a launch has at most 65535 workgroups of 1024 pieces of at least 2 bytes a page)
-  if (page_tokens * row_elems > kMaxPageElems)
-    return set_error(ctx, Q35_ERR_UNSUPPORTED, "cache copy: at most 2^25 values a page");
   if (layers > 1 && layer_stride / row_elems / page_tokens < total_pages)
     return set_error(ctx, Q35_ERR_INVALID, "cache copy: layers overlap");
   return Q35_OK;
