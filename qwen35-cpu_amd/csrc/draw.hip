@@ -45,7 +45,7 @@ constexpr int kBins = 192;    // quarter octaves: a weight below 2^-44 is no who
 constexpr int kListed = 1024; // tokens a slice lists
 // Light rows: without the rule one row of top-k 20 takes 21 instead of 17 us, 256
 // mixed rows 149 instead of 111. A slice lists all that such rows need, but for
-// ties.
+// ties and for a cut in the row's last bin, which takes all that lies further down.
 constexpr int kLightTopK = 512;
 constexpr int kUnitBits = 43;
 constexpr double kUnit = 8796093022208.0;  // 2^43
@@ -266,7 +266,7 @@ struct Picker {
   // The list places of bins g0 .. g1 in every slice (then a barrier).
   __device__ __forceinline__ void places(int g0, int g1) const {
     const int s = threadIdx.x;
-    int first = 0, end = 0;
+    int first = 0, last = 0, end = 0;  // tokens before the range, before its last bin, and through it
     if (s < slices && sh.top[s] != -INFINITY) {
       // the slice's bins: its own bin b is the row's b + below, the last takes
       // all that lies further down (so a range that ends in it, short of the
@@ -274,10 +274,13 @@ struct Picker {
       const int below = sh.below[s], b0 = max(g0 - below, 0), b1 = g1 == kBins - 1 ? kBins - 1 : min(g1 - below, kBins - 2);
       if (b1 >= b0) {
         first = b0 > 0 ? ends[s * kBins + b0 - 1] : 0;
+        last = b1 > b0 ? ends[s * kBins + b1 - 1] : first;
         end = max(first, static_cast<int>(ends[s * kBins + b1]));
       }
     }
-    const bool listed = end <= kListed && !(o.light && first >= o.top_k);
+    // (a light row's slice leaves out each bin behind top_k others: where the row's
+    // last bin takes several of the slice's, the first of them alone says nothing)
+    const bool listed = end <= kListed && !(o.light && last >= o.top_k && end > o.top_k);
     unsigned long long unused = 0ull;
     unsigned through = listed ? end - first : 0;
     running(unused, through);
