@@ -440,9 +440,11 @@ struct Picker {
     places(g, g);
     unsigned long long low = 0ull, high = ~0ull;
     if (n > kSettle && g < kBins - 1) {
-      // keys of values whose x * scale may round into the bin
+      // keys of values whose x * scale may round into the bin: a product is off by
+      // 2^-24 of it, or, below 2^-126, by its whole size (-0 is in the bin of 0)
       const float y = ytop - static_cast<float>(g), x0 = y / o.bin_scale, x1 = (y + 1.0F) / o.bin_scale;
-      const float lo = x0 - fabsf(x0) * 1.0e-6F, hi = x1 + fabsf(x1) * 1.0e-6F;
+      const float tiny = 1.17549435e-38F / o.bin_scale;
+      const float lo = x0 - fabsf(x0) * 1.0e-6F - tiny, hi = x1 + fabsf(x1) * 1.0e-6F + tiny;
       if (lo > -INFINITY && lo < hi && hi < INFINITY) {
         low = argmax_key(lo, 0xffffffffu);
         high = argmax_key(hi, 0u);

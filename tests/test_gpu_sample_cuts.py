@@ -70,3 +70,14 @@ def test_masked_vocabulary(q, ctx, masked):
     x[rng.random(x.shape) < masked] = -np.inf
     for temperature in (0.05, 0.1, 0.3):
         _check(q, ctx, x, rng.random(4).astype(np.float32), temperature, 20, workspace=_filled(q, ctx, 4, vocab, 255))
+
+
+@pytest.mark.parametrize("options", [dict(), dict(top_p=0.3), dict(top_k=4001), dict(top_p=0.77, min_p=0.9)])
+@pytest.mark.parametrize("temperature,size", [(np.inf, 1e-42), (1e30, 1e-17), (1e30, 1e-12), (100.0, 1e-44), (1.0, 1e-44)])
+def test_values_around_zero(q, ctx, temperature, size, options):
+    """Thousands of values so near to zero that their products with the bins'
+    scale round to it, from both sides: every weight is 1."""
+    rng = np.random.default_rng(43)
+    x = (rng.standard_normal((2, 13000)) * size).astype(np.float32)
+    assert (x < 0).sum() > 3000 and (x > 0).sum() > 3000
+    _check(q, ctx, x, np.array([0.902, 0.3117], np.float32), temperature, **options)
