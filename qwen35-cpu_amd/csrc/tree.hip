@@ -36,8 +36,8 @@ constexpr int kGroupVectors = 16;  // query vectors (node, head) per wavefront
 constexpr int kTreeWaves = 8;
 constexpr int kRowStages = kTreeWaves;  // stages whose rows are resolved at once, one per wavefront
 constexpr int kBlockVectors = kTreeWaves * kGroupVectors;  // query vectors per item
-// Probabilities are taken relative to the running maximum less 14 binades: as
-// two binary16 operands (22 bits) they then reach down to 2^-38 of the largest.
+// Probabilities are taken times 2^14, the largest then: as two binary16 operands
+// (22 bits) they reach down to 2^-38 of it.
 constexpr float kProbBinades = 14.0F;
 
 // Products of cache rows and 16 query vectors on v_mfma_f32_16x16x32_f16, with
@@ -49,18 +49,19 @@ constexpr float kProbBinades = 14.0F;
 // tile's token 16(i / 4) + 4(l / 16) + i % 4 on both sides.
 __device__ __forceinline__ int slot_token(int i, int quad) { return 16 * (i >> 2) + 4 * quad + (i & 3); }
 
-// 2^(s * scale - ref), the product rounded on its own: the largest score then
-// meets its own value in ref (a contracted difference would leave the rounding
-// of ref, which an infinite weight could come of where scores are huge).
-__device__ __forceinline__ float score_weight(float s, float scale, float ref) {
+// A score in binades, and its weight 2^(score - top + 14): the product rounded on
+// its own (a contracted difference would leave the rounding of the largest score,
+// which an infinite weight could come of where scores are huge), and the 14 added
+// to the difference (scores from 2^25 on hold no such step: a reference of top -
+// 14 gave weights up to 2^16, past binary16).
+__device__ __forceinline__ float score_of(float s, float scale) {
 #pragma clang fp contract(off)
-  const float x = s * scale;
-  return Q35_EXP2(x - ref);
+  return s * scale;
 }
-__device__ __forceinline__ float score_ref(float s, float scale) {
+__device__ __forceinline__ float score_weight(float s, float scale, float top) {
 #pragma clang fp contract(off)
   const float x = s * scale;
-  return x - kProbBinades;
+  return Q35_EXP2((x - top) + kProbBinades);
 }
 
 struct TreeRequest {
@@ -353,7 +354,7 @@ __global__ __launch_bounds__(64 * kTreeWaves) Q35_WAVES_PER_EU(2) void tree_atte
     q35_f32x4 acc[NV];  // dims 16 n + 4 quad + i of the lane's vector
 #pragma unroll
     for (int n = 0; n < NV; ++n) acc[n] = q35_f32x4{0.0F, 0.0F, 0.0F, 0.0F};
-    // the lane's vector: weights are 2^(score - ref); the sum is over its own tokens
+    // the lane's vector: weights are 2^(score - ref + 14); the sum is over its own tokens
     float ref = -INFINITY, sum = 0.0F;
 
     // 32 rows, K at cache[kb] and V a block behind it, the first of them the
@@ -395,7 +396,7 @@ __global__ __launch_bounds__(64 * kTreeWaves) Q35_WAVES_PER_EU(2) void tree_atte
 #pragma unroll
       for (int i = 0; i < 8; ++i) top = fmaxf(top, s[i >> 2][i & 3]);
       top = q35_max_rows(top);
-      const float next = fmaxf(ref, score_ref(top, sscale)), least = next == -INFINITY ? 0.0F : next;
+      const float next = fmaxf(ref, score_of(top, sscale)), least = next == -INFINITY ? 0.0F : next;
       const float keep = ref == next ? 1.0F : Q35_EXP2(ref - least);  // 0 at the first seen row
       float p[8], sums = 0.0F;
 #pragma unroll
