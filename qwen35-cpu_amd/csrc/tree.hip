@@ -341,7 +341,9 @@ __global__ __launch_bounds__(64 * kTreeWaves) Q35_WAVES_PER_EU(2) void tree_atte
       ex = ex == 0 || ex == 255 ? 127 + 8 : max(ex, 20);
       float down = __uint_as_float(static_cast<uint32_t>(127 + 8 + 127 - ex) << 23);  // 2^(8 - exponent)
       const float up = __uint_as_float(static_cast<uint32_t>(max(ex - 8, 1)) << 23);        // 2^(exponent - 8)
-      sscale = fabsf(a.scale) * 1.44269504088896341F * up;
+      // (neither 0 nor infinite, for products of -inf, of hidden rows, and of 0:
+      // at the least the scores, 2^34 at most before, all round to 0)
+      sscale = fminf(fmaxf(fabsf(a.scale) * 1.44269504088896341F * up, 1.17549435e-38F), 3.40282347e38F);
       if (a.scale < 0.0F) down = -down;  // the scores' order is then that of the products
 #pragma unroll
       for (int kk = 0; kk < KS; ++kk) {

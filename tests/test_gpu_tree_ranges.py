@@ -5,7 +5,6 @@ import numpy as np
 import pytest
 
 from tests.drafted_util import TreeCase
-from tests.test_gpu_tree_attention import _check
 
 pytestmark = pytest.mark.gpu
 
@@ -43,3 +42,36 @@ def test_random_queries_of_large_scores(q, ctx, size):
     case = TreeCase(32, [90, 200], [9, 12], 4, 2, 64, q_scale=size)
     case.scale = 0.125
     assert np.isfinite(case.run(q, ctx)).all()
+
+
+def _check_scale(q, ctx, case, scale):
+    """_check for a scale of either sign (the formula of -scale is that of -q)."""
+    case.scale = scale
+    got = case.run(q, ctx).astype(np.float64)
+    case.scale = abs(scale)
+    if scale < 0:
+        case.q = -case.q
+    want, tol = case.expected()
+    assert np.isfinite(want).all() and np.isfinite(got).all()
+    assert (np.abs(got - want) <= tol).all(), np.max(np.abs(got - want) / np.maximum(tol, 1e-300))
+
+
+@pytest.mark.parametrize("scale,q_scale", [(0.0, 1.0), (-0.0, 1.0), (0.0, 1e-30), (1e-25, 1e-25), (-1e-25, 1e-25), (1e-38, 1e-36),
+                                           (1e-44, 1.0), (1e-44, 1e-30), (-1e-30, 1e-9)])
+def test_scales_that_vanish(q, ctx, scale, q_scale):
+    """Scores of zero, or that round to it: an even average over the seen rows,
+    in tiles that hold hidden rows and in others."""
+    _check_scale(q, ctx, TreeCase(33, [10, 70, 0, 700], [3, 9, 5, 2], 4, 2, 64, q_scale=q_scale), scale)
+
+
+@pytest.mark.parametrize("scale", [-0.2, -1.0])
+def test_negative_scale(q, ctx, scale):
+    _check_scale(q, ctx, TreeCase(34, [10, 70, 700], [3, 9, 2], 4, 2, 64), scale)
+
+
+@pytest.mark.parametrize("scale,q_scale", [(3e38, 0.0), (3e38, 1e4), (1e38, 1e30), (-3e38, 1e4)])
+def test_scales_that_overflow(q, ctx, scale, q_scale):
+    """Keys of zero, or queries: a score of zero is one whatever the scale."""
+    case = TreeCase(35, [10, 70], [3, 9], 4, 2, 64, q_scale=q_scale)
+    case.k[~np.isnan(case.k)] = 0.0
+    _check_scale(q, ctx, case, scale)
