@@ -337,13 +337,24 @@ __global__ __launch_bounds__(64 * kTreeWaves) Q35_WAVES_PER_EU(2) void tree_atte
 #pragma unroll
         for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(raw[kk][i >> 2][i & 3]));
       top = q35_max_rows(top);
+      // (after a lift by 2^60 where it is below 2^-100, subnormal or near it)
+      const bool small = top < 0x1p-100F;
+      if (q35_ballot(small) != 0ull) {
+        const float lift = small ? 0x1p60F : 1.0F;
+        top *= lift;
+#pragma unroll
+        for (int kk = 0; kk < KS; ++kk)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) raw[kk][i] *= lift;
+      }
       int ex = static_cast<int>(__float_as_uint(top) >> 23);  // biased
-      ex = ex == 0 || ex == 255 ? 127 + 8 : max(ex, 20);
+      if (ex == 0 || ex == 255) ex = 127 + 8;
       float down = __uint_as_float(static_cast<uint32_t>(127 + 8 + 127 - ex) << 23);  // 2^(8 - exponent)
-      const float up = __uint_as_float(static_cast<uint32_t>(max(ex - 8, 1)) << 23);        // 2^(exponent - 8)
+      const float up = __uint_as_float(static_cast<uint32_t>(ex - 8) << 23);            // 2^(exponent - 8)
       // (neither 0 nor infinite, for products of -inf, of hidden rows, and of 0:
       // at the least the scores, 2^34 at most before, all round to 0)
-      sscale = fminf(fmaxf(fabsf(a.scale) * 1.44269504088896341F * up, 1.17549435e-38F), 3.40282347e38F);
+      sscale = fabsf(a.scale) * up * (small ? 0x1p-60F : 1.0F) * 1.44269504088896341F;
+      sscale = fminf(fmaxf(sscale, 0x1p-126F), 3.40282347e38F);
       if (a.scale < 0.0F) down = -down;  // the scores' order is then that of the products
 #pragma unroll
       for (int kk = 0; kk < KS; ++kk) {

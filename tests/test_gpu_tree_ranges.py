@@ -75,3 +75,9 @@ def test_scales_that_overflow(q, ctx, scale, q_scale):
     case = TreeCase(35, [10, 70], [3, 9], 4, 2, 64, q_scale=q_scale)
     case.k[~np.isnan(case.k)] = 0.0
     _check_scale(q, ctx, case, scale)
+
+
+@pytest.mark.parametrize("scale,q_scale", [(1e37, 1e-38), (3e37, 1e-41), (-1e38, 1e-43), (1e30, 1e-31), (3e30, 1e-30)])
+def test_queries_of_the_smallest_size(q, ctx, scale, q_scale):
+    """Queries down to fp32's smallest, brought to scores of ordinary size by the scale."""
+    _check_scale(q, ctx, TreeCase(36, [60, 200], [5, 9], 4, 2, 64, q_scale=q_scale), scale)
