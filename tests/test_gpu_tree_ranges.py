@@ -4,7 +4,7 @@ underflow, values that are not finite in requests cut into several parts."""
 import numpy as np
 import pytest
 
-from tests.drafted_util import TreeCase
+from tests.drafted_util import TreeCase, ancestor_bits, random_tree
 
 pytestmark = pytest.mark.gpu
 
@@ -81,3 +81,62 @@ def test_scales_that_overflow(q, ctx, scale, q_scale):
 def test_queries_of_the_smallest_size(q, ctx, scale, q_scale):
     """Queries down to fp32's smallest, brought to scores of ordinary size by the scale."""
     _check_scale(q, ctx, TreeCase(36, [60, 200], [5, 9], 4, 2, 64, q_scale=q_scale), scale)
+
+
+def _check_specials(q, ctx, case, at, where):
+    """The case with values that are not finite in drafted nodes' rows ((request,
+    node, KV head, dim): value): nodes that do not see them as without them, the
+    others' values as the formula's, or NaN where a key is NaN."""
+    clean, tol = case.expected()
+    pool = case.k if where == "k" else case.v
+    seen = np.zeros((case.rows, case.heads), bool)
+    group = case.heads // case.kv_heads
+    for (b, j, g, dim), value in at.items():
+        t = int(case.contexts[b]) + j
+        pool[case.table[b, t // case.page_tokens], t % case.page_tokens, g, dim] = value
+        rows = case.start[b] + np.flatnonzero(np.asarray(case.bits[b])[:, j])
+        seen[rows, group * g:group * (g + 1)] = True
+    print(f"special values in {where}: {at}", flush=True)
+    got = case.run(q, ctx).astype(np.float64)
+    assert (np.abs(got - clean) <= tol)[~seen].all()
+    if where == "v":
+        with np.errstate(invalid="ignore"):
+            want, _ = case.expected()
+        finite = np.isfinite(want)
+        np.testing.assert_array_equal(np.isfinite(got), finite)
+        np.testing.assert_array_equal(got[~finite], want[~finite])  # inf, -inf and NaN each in their place
+        assert (np.abs(got - clean) <= tol)[finite].all()
+    else:
+        assert np.isnan(got[seen]).all()
+
+
+# trees that end inside a stage of 64 rows, cross its border, begin at one, and
+# lie behind several stages
+@pytest.mark.parametrize("where", ["k", "v"])
+@pytest.mark.parametrize("context", [0, 43, 62, 64, 125, 300])
+def test_special_values_in_parts(q, ctx, context, where):
+    parents = np.array([-1, 0, 0, 1, 2, 4], np.int32)
+    for j in (0, 2, 5):
+        case = TreeCase(37, [context], [6], 4, 2, 64, bits=[ancestor_bits(parents)])
+        _check_specials(q, ctx, case, {(0, j, 1, 5): np.nan}, where)
+
+
+@pytest.mark.parametrize("context", [0, 20, 130])
+@pytest.mark.parametrize("head_dim", [64, 256])
+def test_special_values_in_a_wide_tree(q, ctx, context, head_dim):
+    """Infinities of both signs and NaN in nodes of different stages, where one
+    node may see several of them."""
+    rng = np.random.default_rng(6)
+    case = TreeCase(38, [context, 7], [140, 3], 4, 2, head_dim, bits=[ancestor_bits(random_tree(rng, n)) for n in (140, 3)])
+    at = {(0, 3, 0, 9): np.inf, (0, 40, 0, 9): -np.inf, (0, 41, 0, 33): np.inf, (0, 90, 1, 2): np.nan, (0, 139, 1, 63): -np.inf}
+    _check_specials(q, ctx, case, at, "v")
+
+
+def test_special_values_in_many_requests(q, ctx):
+    """More items than workgroups: some are finished where they begin, some in parts."""
+    rng = np.random.default_rng(7)
+    contexts, nodes = rng.integers(0, 90, size=40), rng.integers(1, 9, size=40)
+    case = TreeCase(39, contexts, nodes, 16, 8, 64)
+    at = {(b, int(rng.integers(0, nodes[b])), int(rng.integers(0, 8)), int(rng.integers(0, 64))): v
+          for b, v in zip(range(0, 40, 2), [np.inf, -np.inf, np.nan, np.inf] * 5)}
+    _check_specials(q, ctx, case, at, "v")
