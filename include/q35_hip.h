@@ -180,7 +180,7 @@ int q35_attention_decode_paged(q35_context *ctx, const float *q, const float *ga
  * sigmoid(gate); a node that sees nothing, or whose scores are all -inf, gets
  * zero. Infinite or NaN keys and values reach only the nodes that see their
  * row (a key, or a context row's value, that is not finite may leave NaN in
- * those).
+ * those). Scores have to fit fp32, in units of binades.
  *   head_dim 64, 128 or 256; heads a multiple of kv_heads; page_tokens a power
  *   of two; at most 256 nodes a request; FP16 pools of total_pages pages;
  *   16-byte aligned buffers; pools, table and masks are not written.

@@ -150,8 +150,8 @@ extern "C" int q35_attention_tree_workspace(q35_context *ctx, size_t batch, size
     if (bytes == nullptr) return set_error(ctx, Q35_ERR_INVALID, "tree attention: no place for the size");
     TreeArgs a;
     const int st = tree_check(ctx, batch, rows, max_nodes, max_len, heads, kv_heads, head_dim, &a);
-    size_t specials = 0, part_o = 0, part_ml = 0;
-    if (st == Q35_OK) *bytes = tree_workspace_bytes(a, &specials, &part_o, &part_ml);
+    size_t part_o = 0, part_ml = 0;
+    if (st == Q35_OK) *bytes = tree_workspace_bytes(a, &part_o, &part_ml);
     return st;
   });
 }
@@ -181,8 +181,8 @@ extern "C" int q35_attention_tree_paged(q35_context *ctx, const float *q, const 
     if (!std::isfinite(scale)) return set_error(ctx, Q35_ERR_INVALID, "tree attention: scale is not finite");
     if (rows == 0) return Q35_OK;
     void *work = nullptr;
-    size_t specials = 0, part_o = 0, part_ml = 0;
-    st = workspace_get(ctx, workspace, workspace_bytes, tree_workspace_bytes(a, &specials, &part_o, &part_ml), &work);
+    size_t part_o = 0, part_ml = 0;
+    st = workspace_get(ctx, workspace, workspace_bytes, tree_workspace_bytes(a, &part_o, &part_ml), &work);
     if (st != Q35_OK) return st;
     a.q = q;
     a.gates = gates;
@@ -199,7 +199,6 @@ extern "C" int q35_attention_tree_paged(q35_context *ctx, const float *q, const 
     a.out = output;
     a.scale = scale;
     a.first_units = static_cast<long long *>(work);
-    a.specials = reinterpret_cast<int32_t *>(static_cast<char *>(work) + specials);
     a.part_o = reinterpret_cast<float *>(static_cast<char *>(work) + part_o);
     a.part_ml = reinterpret_cast<float *>(static_cast<char *>(work) + part_ml);
     const hipError_t e = launch_tree_attention(a, ctx->stream);

@@ -484,7 +484,6 @@ struct TreeArgs {
   float scale = 1.0F;
   int groups = 1;                                // workgroups (tree_groups)
   long long *first_units = nullptr;              // [batch + 1] work units before each request
-  int32_t *specials = nullptr;                   // two per workgroup: node values that are not finite in a part
   float *part_o = nullptr, *part_ml = nullptr;   // two parts per workgroup: [..][head_dim], [..][2] (max, sum)
 };
 // Work units of a request at most: below 2^31 for a launch, and all requests' at
@@ -492,8 +491,8 @@ struct TreeArgs {
 constexpr long long kMaxTreeUnits = 1LL << 43;
 long long tree_request_units(int max_nodes, int max_len, int heads, int kv_heads);
 int tree_groups(int batch, int max_nodes, int max_len, int heads, int kv_heads, int cu_count);
-// Workspace bytes, and where specials, part_o and part_ml lie in it (first_units at 0).
-size_t tree_workspace_bytes(const TreeArgs &a, size_t *specials, size_t *part_o, size_t *part_ml);
+// Workspace bytes, and where part_o and part_ml lie in it (first_units at 0).
+size_t tree_workspace_bytes(const TreeArgs &a, size_t *part_o, size_t *part_ml);
 hipError_t launch_tree_attention(const TreeArgs &a, hipStream_t stream);
 
 struct AcceptArgs {

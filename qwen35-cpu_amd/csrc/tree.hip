@@ -150,37 +150,26 @@ __device__ __forceinline__ int unit_group(long long unit, long long total, int g
   return static_cast<int>(floor(static_cast<double>((unit + 1) * groups - 1) / static_cast<double>(total)));
 }
 
-// The formula row by row over the rows that a node sees, one wavefront for one
-// (node, head): for items with values that are not finite among their nodes.
+// Four dims (from dim 4 f on) of a node's unnormalised output, and the values
+// that are not finite in the rows of nodes j0 .. j1 - 1 it sees (`special`: a bit
+// for each node with such values), which the products had as zeros: a row that
+// weighs anything makes such a sum the value itself.
 template <int HD>
-__device__ void tree_row_by_row(const TreeArgs &a, const TreeRequest &rq, int i, int h, int b) {
-  constexpr int F = HD / 4;  // lanes past the dims repeat them
-  const int f = threadIdx.x & (F - 1), g = h / (a.heads / a.kv_heads);
-  const size_t kvw = static_cast<size_t>(a.kv_heads) * HD, head = (static_cast<size_t>(rq.row0 + i) * a.heads + h) * HD + 4 * f;
-  const int32_t *table = a.page_table + static_cast<size_t>(b) * a.max_pages;
-  const uint64_t *words = a.masks + static_cast<size_t>(rq.row0 + i) * a.mask_words;
-  const q35_f32x4 x = *reinterpret_cast<const q35_f32x4 *>(a.q + head);
-  q35_f32x4 o = {0.0F, 0.0F, 0.0F, 0.0F};
-  float mx = -INFINITY, l = 0.0F;
-  for (int t = 0; t < rq.len; ++t) {
-    const int j = t - rq.context;
-    if (j >= 0 && !((words[j >> 6] >> (j & 63)) & 1ull)) continue;
-    const int page = table[t >> a.page_shift];
-    const bool ok = static_cast<unsigned>(page) < static_cast<unsigned>(a.total_pages);
-    const size_t at = static_cast<size_t>(((ok ? page : 0) << a.page_shift) + (t & ((1 << a.page_shift) - 1))) * kvw +
-                      static_cast<size_t>(g) * HD + 4 * f;
-    float dot = 0.0F;
+__device__ __forceinline__ q35_f32x4 tree_add_special(const TreeArgs &a, const TreeRequest &rq, int b, int g, int node, int f,
+                                                      const uint32_t *special, int j0, int j1, q35_f32x4 y) {
+  const uint64_t *words = a.masks + static_cast<size_t>(rq.row0 + node) * a.mask_words;
+#pragma unroll 1
+  for (int j = j0; j < j1; ++j) {
+    if (!((special[j >> 5] >> (j & 31)) & 1u) || !((words[j >> 6] >> (j & 63)) & 1ull)) continue;
+    const int t = rq.context + j, page = a.page_table[static_cast<size_t>(b) * a.max_pages + (t >> a.page_shift)];
+    if (static_cast<unsigned>(page) >= static_cast<unsigned>(a.total_pages)) continue;  // NaN as it is
+    const uint16_t *v = a.v_pool + static_cast<size_t>((page << a.page_shift) + (t & ((1 << a.page_shift) - 1))) * a.kv_heads * HD +
+                        static_cast<size_t>(g) * HD + 4 * f;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) dot = fmaf(x[e], half_bits_to_float(a.k_pool[at + e]), dot);
-    const float s = ok ? group_sum<F>(dot) * (a.scale * 1.44269504088896341F) : NAN;
-    const float next = fmaxf(mx, s), least = next == -INFINITY ? 0.0F : next;
-    const float keep = mx == next ? 1.0F : Q35_EXP2(mx - least), p = Q35_EXP2(s - least);
-    mx = next;
-    l = fmaf(l, keep, p);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] = fmaf(p, half_bits_to_float(a.v_pool[at + e]), o[e] * keep);
+    for (int e = 0; e < 4; ++e)
+      if ((v[e] & 0x7c00u) == 0x7c00u) y[e] += half_bits_to_float(v[e]);
   }
-  tree_store(a.out + head, o, l, a.gates != nullptr, tree_gate(a.gates, head));
+  return y;
 }
 
 // One workgroup of eight wavefronts. A stage's K and V rows go straight from
@@ -217,6 +206,7 @@ __global__ __launch_bounds__(64 * kTreeWaves) Q35_WAVES_PER_EU(2) void tree_atte
     long long units[kTreeWaves];
     long long first_unit;
     int first_request, special;
+    uint32_t special_nodes[kMaxTreeNodes / 32];
   } sh;
   uint16_t *cache = sh.cache;
   const int tid = threadIdx.x, wave = q35_uniform(tid >> 6), lane = tid & 63, col = lane & 15, quad = lane >> 4;
@@ -261,6 +251,7 @@ __global__ __launch_bounds__(64 * kTreeWaves) Q35_WAVES_PER_EU(2) void tree_atte
 
   int b = sh.first_request;
   long long base = sh.first_unit;  // the request's first unit
+  bool again = false;  // the item's stages once more, its nodes' values that are not finite as zeros
   for (long long unit = begin; unit < end;) {
     const TreeRequest rq = tree_request(a, b);
     const int stages = item_stages(rq), blocks = item_blocks(a, rq);
@@ -320,7 +311,8 @@ __global__ __launch_bounds__(64 * kTreeWaves) Q35_WAVES_PER_EU(2) void tree_atte
         Q35_LOAD_LDS16(vp + row + 8 * (slot ^ (2 * r & (PIECES - 1))), to + BLOCK);
       }
     };
-    if (tid == 0) sh.special = 0;
+    if (!again && tid == 0) sh.special = 0;
+    if (again && tid < kMaxTreeNodes / 32) sh.special_nodes[tid] = 0u;
     keep_rows(0, run_page(0));
     int following = run_page(1);
     lds_barrier();
@@ -458,18 +450,31 @@ __global__ __launch_bounds__(64 * kTreeWaves) Q35_WAVES_PER_EU(2) void tree_atte
       const int t = kStageTokens * s;
       if (t + kStageTokens > rq.context) {
         // An infinite or NaN value in a node's row: products with weights of 0
-        // would carry it to nodes that do not see the row, so such an item is
-        // computed anew, row by row.
+        // would carry it to nodes that do not see the row. Where there is one the
+        // stages are gone through again, with zeros in the place of such values
+        // (rows past the request, copies of a stage's first, among them).
+        const int value = (s & 1) * 2 * BLOCK + BLOCK + 8 * tid, first = t - rq.context + tid / PIECES;
         bool special = false;
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
-          const int e = i * 64 * kTreeWaves + tid, r = t + e / PIECES;
-          const q35_u32x4 v = *reinterpret_cast<const q35_u32x4 *>(cache + (s & 1) * 2 * BLOCK + BLOCK + 8 * e);
+          const int j = first + i * 64 * kTreeWaves / PIECES;
+          const q35_u32x4 v = *reinterpret_cast<const q35_u32x4 *>(cache + value + 8 * i * 64 * kTreeWaves);
 #pragma unroll
           for (int d = 0; d < 4; ++d)
-            special |= r >= rq.context && r < rq.len && ((v[d] & 0x7c00u) == 0x7c00u || (v[d] & 0x7c000000u) == 0x7c000000u);
+            special |= j >= 0 && j < rq.nodes && ((v[d] & 0x7c00u) == 0x7c00u || (v[d] & 0x7c000000u) == 0x7c000000u);
         }
         if (special) sh.special = 1;
+        if (again) {
+#pragma unroll 1
+          for (int e = 0; e < 8 * LOADS; ++e) {
+            const int j = first + (e >> 3) * 64 * kTreeWaves / PIECES;
+            uint16_t *v = cache + value + 8 * (e >> 3) * 64 * kTreeWaves + (e & 7);
+            if (j < 0 || (*v & 0x7c00u) != 0x7c00u) continue;
+            *v = 0;
+            if (j < rq.nodes) atomicOr(&sh.special_nodes[j >> 5], 1u << (j & 31));
+          }
+          lds_barrier();
+        }
       }
       if (active) {
         for (int k = 0; k < 2; ++k)
@@ -478,6 +483,11 @@ __global__ __launch_bounds__(64 * kTreeWaves) Q35_WAVES_PER_EU(2) void tree_atte
       }
     }
     lds_barrier();  // every wavefront is done with the last stage
+    if (sh.special != 0 && !again) {
+      again = true;
+      unit -= u1 - u0;
+      continue;
+    }
 
     // Each group's vectors through LDS, [vector][dims] with the 16-byte pieces of
     // a row at their number xor the vector, whose rows then leave whole, dealt
@@ -499,26 +509,22 @@ __global__ __launch_bounds__(64 * kTreeWaves) Q35_WAVES_PER_EU(2) void tree_atte
     }
     lds_barrier();
     const int count = min(kBlockVectors, vectors - m0);
-    if (sh.special != 0 && whole) {
-      for (int v = wave; v < count; v += kTreeWaves) {
-        const int vn = (m0 + v) / qpk;
-        tree_row_by_row<HD>(a, rq, vn, g * qpk + m0 + v - vn * qpk, b);
-      }
-    } else {
-      const int f = lane & (F - 1);
+    const int f = lane & (F - 1);
 #pragma unroll 4
-      for (int v = wave * (64 / F) + lane / F; v < count; v += kTreeWaves * (64 / F)) {
-        const q35_f32x4 y = reinterpret_cast<q35_f32x4 *>(cache)[v * F + (f ^ (v & (kGroupVectors - 1)))];
-        if (whole) {
-          const int vn = (m0 + v) / qpk, vu = m0 + v - vn * qpk;
-          const size_t to = (static_cast<size_t>(rq.row0 + vn) * a.heads + g * qpk + vu) * HD + 4 * f;
-          tree_store(a.out + to, y, sh.sums[v / kGroupVectors][v & (kGroupVectors - 1)], a.gates != nullptr, tree_gate(a.gates, to));
-        } else {
-          *reinterpret_cast<q35_f32x4 *>(a.part_o + (place + v) * HD + 4 * f) = y;
-        }
+    for (int v = wave * (64 / F) + lane / F; v < count; v += kTreeWaves * (64 / F)) {
+      q35_f32x4 y = reinterpret_cast<q35_f32x4 *>(cache)[v * F + (f ^ (v & (kGroupVectors - 1)))];
+      const int vn = (m0 + v) / qpk, vu = m0 + v - vn * qpk;
+      if (again)
+        y = tree_add_special<HD>(a, rq, b, g, vn, f, sh.special_nodes, max(kStageTokens * s0 - rq.context, 0),
+                                 min(kStageTokens * s1 - rq.context, rq.nodes), y);
+      if (whole) {
+        const size_t to = (static_cast<size_t>(rq.row0 + vn) * a.heads + g * qpk + vu) * HD + 4 * f;
+        tree_store(a.out + to, y, sh.sums[v / kGroupVectors][v & (kGroupVectors - 1)], a.gates != nullptr, tree_gate(a.gates, to));
+      } else {
+        *reinterpret_cast<q35_f32x4 *>(a.part_o + (place + v) * HD + 4 * f) = y;
       }
     }
-    if (!whole && tid == 0) a.specials[2 * w + (s0 == 0 ? 1 : 0)] = sh.special;
+    again = false;
     lds_barrier();  // the results and the row lists are free for the next item
   }
 }
@@ -561,18 +567,12 @@ __global__ __launch_bounds__(64) void tree_merge_kernel(TreeArgs a) {
     for (int u = 0; u < U; ++u) x[u] = *reinterpret_cast<const q35_f32x4 *>(a.part_o + place(min(first_part + u, w1)) * HD + 4 * f);
   };
   q35_f32x2 ml = *reinterpret_cast<const q35_f32x2 *>(a.part_ml + 2 * place(min(w0 + lane, w1)));
-  bool special = false;
-  for (int w = w0 + lane; w <= w1; w += 64) special |= a.specials[2 * w + (w == w0 ? 1 : 0)] != 0;
   ask(w0);
   const q35_f32x4 gate = tree_gate(a.gates, head);
   q35_compiler_fence();
   float top = ml[0];
   for (int w = w0 + lane + 64; w <= w1; w += 64) top = fmaxf(top, a.part_ml[2 * place(w)]);
   top = group_max<64>(top);
-  if (q35_ballot(special) != 0ull) {
-    tree_row_by_row<HD>(a, rq, i, h, b);
-    return;
-  }
   const float least = top == -INFINITY ? 0.0F : top;
   q35_f32x4 o = {0.0F, 0.0F, 0.0F, 0.0F};
   float l = 0.0F;
@@ -669,11 +669,10 @@ long long tree_request_units(int max_nodes, int max_len, int heads, int kv_heads
   return blocks * kv_heads * ((static_cast<long long>(max_len) + kStageTokens - 1) / kStageTokens + kItemUnits);
 }
 
-size_t tree_workspace_bytes(const TreeArgs &a, size_t *specials, size_t *part_o, size_t *part_ml) {
+size_t tree_workspace_bytes(const TreeArgs &a, size_t *part_o, size_t *part_ml) {
   auto align = [](size_t n) { return (n + 255) & ~static_cast<size_t>(255); };
   const size_t parts = 2 * static_cast<size_t>(a.groups) * kBlockVectors;
-  *specials = align((static_cast<size_t>(a.batch) + 1) * 8);
-  *part_o = *specials + align(2 * static_cast<size_t>(a.groups) * 4);
+  *part_o = align((static_cast<size_t>(a.batch) + 1) * 8);
   *part_ml = *part_o + align(parts * a.head_dim * 4);
   return *part_ml + align(parts * 8);
 }

@@ -210,14 +210,9 @@ inline T __shfl_xor(T v, int mask, int width = 64) {
   return ::q35emu::shfl_xor(v, mask);
 }
 inline unsigned atomicAdd(unsigned *p, unsigned v) { return __atomic_fetch_add(p, v, __ATOMIC_SEQ_CST); }
+inline unsigned atomicOr(unsigned *p, unsigned v) { return __atomic_fetch_or(p, v, __ATOMIC_SEQ_CST); }
 inline unsigned long long atomicAdd(unsigned long long *p, unsigned long long v) {
   return __atomic_fetch_add(p, v, __ATOMIC_SEQ_CST);
-}
-inline unsigned long long atomicMin(unsigned long long *p, unsigned long long v) {
-  unsigned long long cur = __atomic_load_n(p, __ATOMIC_SEQ_CST);
-  while (cur > v && !__atomic_compare_exchange_n(p, &cur, v, false, __ATOMIC_SEQ_CST, __ATOMIC_SEQ_CST)) {
-  }
-  return cur;
 }
 inline unsigned long long atomicMax(unsigned long long *p, unsigned long long v) {
   unsigned long long cur = __atomic_load_n(p, __ATOMIC_SEQ_CST);

@@ -4,7 +4,7 @@ underflow, values that are not finite in requests cut into several parts."""
 import numpy as np
 import pytest
 
-from tests.drafted_util import TreeCase, ancestor_bits, random_tree
+from tests.drafted_util import EMULATED, TreeCase, ancestor_bits, random_tree
 
 pytestmark = pytest.mark.gpu
 
@@ -140,3 +140,27 @@ def test_special_values_in_many_requests(q, ctx):
     at = {(b, int(rng.integers(0, nodes[b])), int(rng.integers(0, 8)), int(rng.integers(0, 64))): v
           for b, v in zip(range(0, 40, 2), [np.inf, -np.inf, np.nan, np.inf] * 5)}
     _check_specials(q, ctx, case, at, "v")
+
+
+@pytest.mark.skipif(EMULATED, reason="times need the device")
+def test_time_with_special_values(q, ctx):
+    """A drafted node's value that is not finite has the stages around it gone
+    through twice: 47 against 36 us here. Row by row such an item took 12.7 ms."""
+    times = []
+    for value in (1.0, np.nan):
+        case = TreeCase(40, [16000], [5], 8, 2, 256)
+        t = 16000 + 2
+        case.v[case.table[0, t // 16], t % 16, 1, 5] = value
+        d = case.device(ctx)
+        print(f"tree attention of 16000 rows, a value of {value}", flush=True)
+        for _ in range(3):
+            case.call(q, ctx, d)
+        best = np.inf
+        for _ in range(5):
+            ctx.timer_begin()
+            for _ in range(5):
+                case.call(q, ctx, d)
+            best = min(best, ctx.timer_end() * 200.0)
+        times.append(best)
+    print(times)
+    assert times[1] < 2.5 * times[0], times
