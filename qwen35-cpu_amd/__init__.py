@@ -333,7 +333,10 @@ class Context:
     """One device, one stream (replaces the reference CpuExecutor)."""
 
     def __init__(self, device: int = 0, stream=None):
-        """stream: a hipStream_t (as an integer) to run on, None: one of its own."""
+        """stream: a hipStream_t (as an integer) to run on, None: one of its own. The default stream (0, torch's
+        current one unless it was changed) is refused: no calls can be captured on it."""
+        if stream is not None and not getattr(stream, "value", stream):
+            raise ValueError("Context: the default stream cannot be used; pass another one, or None for one of its own")
         h = c_void_p()
         _check(lib.q35_context_create(device, stream, ctypes.byref(h)), "context create")
         self.handle = h
