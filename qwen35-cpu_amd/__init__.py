@@ -500,7 +500,13 @@ def sample_logits(ctx, logits, stride, counts, penalties, temperatures, top_k, t
 
 
 def _page_list(a):
-    return np.ascontiguousarray(a, np.int32)
+    """Page or row numbers on the host as int32; what int32 does not hold is refused, not cut to it."""
+    given = np.asarray(a)
+    with np.errstate(invalid="ignore"):
+        out = np.ascontiguousarray(given, np.int32)
+    if given.dtype != np.int32 and not np.array_equal(out, given):
+        raise ValueError("page and token numbers are whole numbers of 32 bits")
+    return out
 
 
 def cache_copy_pages(ctx, k_pool, v_pool, layers, layer_stride, total_pages, page_tokens, row_elems, src, dst, tokens=None):
@@ -674,7 +680,7 @@ class Runtime(_Profiled):
     def page_fork(self, pages, tokens, children=1):
         """Page lists [children][len(pages)] of continuations of `tokens` positions: full pages shared, a partly
         filled last page copied for each."""
-        pages = np.ascontiguousarray(pages, np.int32)
+        pages = _page_list(pages)
         out = np.zeros((children, pages.size), np.int32)
         self.ctx.check(lib.q35_page_fork(self.handle, _ptr(pages), pages.size, tokens, children, _ptr(out)), "page fork")
         return out
