@@ -249,6 +249,8 @@ int q35_sample_logits(q35_context *ctx, const float *logits, size_t stride, cons
 /* ------------------------------------------------- copies inside the cache
  * K/V pools of `layers` layers, layer_stride elements apart, each
  * [total_pages][page_tokens][row_elems] FP16 (row_elems = kv_heads * head_dim).
+ * The pools' layers may alternate in memory, but not overlap (copies take one
+ * pool for both).
  *
  * q35_cache_copy_pages: rows [0, tokens[i]) of page src_pages[i] to page
  * dst_pages[i] in every layer (tokens NULL: whole pages), KvPagesF16's copy on

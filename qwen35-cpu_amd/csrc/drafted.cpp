@@ -108,9 +108,23 @@ int draw_check(q35_context *ctx, size_t rows, size_t vocab) {
   return Q35_OK;
 }
 
-// Pools of the cache copies: addresses and sizes.
+// Whether a layer of one pool shares memory with a layer of the other: their
+// distance less a whole number of layer strides is below a layer's size.
+bool pools_overlap(const void *k, const void *v, size_t layers, size_t layer_stride, size_t layer_elems) {
+  const __int128 distance = static_cast<__int128>(reinterpret_cast<uintptr_t>(v)) - reinterpret_cast<uintptr_t>(k);
+  const __int128 size = 2 * static_cast<__int128>(layer_elems), stride = layers > 1 ? 2 * static_cast<__int128>(layer_stride) : size;
+  const __int128 most = static_cast<__int128>(layers) - 1;
+  for (__int128 m = distance / stride - 1; m <= distance / stride + 1; ++m) {
+    const __int128 rest = distance - std::clamp(m, -most, most) * stride;
+    if (rest < size && -rest < size) return true;
+  }
+  return false;
+}
+
+// Pools of the cache copies: addresses and sizes. One pool for K and V is `same`
+// (copies write the same bytes twice then, but moves would be made twice).
 int pool_check(q35_context *ctx, const void *k, const void *v, size_t layers, size_t layer_stride, size_t total_pages,
-               size_t page_tokens, size_t row_elems) {
+               size_t page_tokens, size_t row_elems, bool same) {
   if (k == nullptr || v == nullptr || layers == 0 || total_pages == 0 || page_tokens == 0 || row_elems == 0 ||
       !aligned(k, 2) || !aligned(v, 2))
     return set_error(ctx, Q35_ERR_INVALID, "cache copy: a missing pool or an empty shape");
@@ -118,6 +132,8 @@ int pool_check(q35_context *ctx, const void *k, const void *v, size_t layers, si
     return set_error(ctx, Q35_ERR_UNSUPPORTED, "cache copy: at most 2^31 - 1 cache rows of 2^20 values");
   if (layers > 1 && layer_stride / row_elems / page_tokens < total_pages)
     return set_error(ctx, Q35_ERR_INVALID, "cache copy: layers overlap");
+  if (!(same && k == v) && pools_overlap(k, v, layers, layer_stride, total_pages * page_tokens * row_elems))
+    return set_error(ctx, Q35_ERR_INVALID, "cache copy: the K and V pools overlap");
   return Q35_OK;
 }
 
@@ -281,7 +297,7 @@ extern "C" int q35_cache_copy_pages(q35_context *ctx, uint16_t *k_pool, uint16_t
                                     const int32_t *src_pages, const int32_t *dst_pages, const int32_t *tokens,
                                     size_t count) {
   return guarded(ctx, [&]() -> int {
-    const int st = pool_check(ctx, k_pool, v_pool, layers, layer_stride, total_pages, page_tokens, row_elems);
+    const int st = pool_check(ctx, k_pool, v_pool, layers, layer_stride, total_pages, page_tokens, row_elems, true);
     if (st != Q35_OK || count == 0) return st;
     if (src_pages == nullptr || dst_pages == nullptr)
       return set_error(ctx, Q35_ERR_INVALID, "page copy: no pages given");
@@ -328,7 +344,7 @@ extern "C" int q35_cache_compact_rows(q35_context *ctx, uint16_t *k_pool, uint16
                                       const int32_t *path, size_t path_stride, const int32_t *path_count,
                                       size_t batch) {
   return guarded(ctx, [&]() -> int {
-    const int st = pool_check(ctx, k_pool, v_pool, layers, layer_stride, total_pages, page_tokens, row_elems);
+    const int st = pool_check(ctx, k_pool, v_pool, layers, layer_stride, total_pages, page_tokens, row_elems, false);
     if (st != Q35_OK || batch == 0) return st;
     if (page_table == nullptr || context_lens == nullptr || path == nullptr || path_count == nullptr || max_pages == 0 ||
         path_stride == 0)
