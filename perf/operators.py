@@ -100,6 +100,21 @@ def draw(rng):
 # ------------------------------------------------------------------- material
 
 
+_PROGRAM = {}
+
+
+def _stream():
+    """The program's one stream, torch's current one from here on and the context's: inputs, operators and whatever
+    reads the outputs follow one another on it."""
+    if "stream" not in _PROGRAM:
+        _PROGRAM["stream"] = torch.cuda.Stream()
+    stream, current = _PROGRAM["stream"], torch.cuda.current_stream()
+    if current != stream:
+        stream.wait_stream(current)
+        torch.cuda.set_stream(stream)
+    return stream
+
+
 def _generators(seed):
     g = torch.Generator(device="cuda")
     g.manual_seed(int(seed) & 0x7FFFFFFF)
@@ -162,6 +177,7 @@ def _halves(g, *shape):
 
 
 def prepare(case, seed):
+    _stream()
     g, r = _generators(seed)
     kind = case["kind"]
     s = {"case": case, "kind": kind}
@@ -355,16 +371,13 @@ def _plain_compact(s):
 # ------------------------------------------------------------- the framework's
 
 
-_PROGRAM = {}
-
-
 def _program():
-    """The package and the program's one context (one device, one stream)."""
-    if not _PROGRAM:
+    """The package and the program's one context (one device, the program's stream)."""
+    if "ctx" not in _PROGRAM:
         import importlib
 
         q = importlib.import_module("qwen35-cpu_amd")
-        _PROGRAM["q"], _PROGRAM["ctx"] = q, q.Context(0)
+        _PROGRAM["q"], _PROGRAM["ctx"] = q, q.Context(0, _stream().cuda_stream)
     return _PROGRAM["q"], _PROGRAM["ctx"]
 
 
