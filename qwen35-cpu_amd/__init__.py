@@ -499,12 +499,17 @@ def sample_logits(ctx, logits, stride, counts, penalties, temperatures, top_k, t
                                     _opt(out_probability), work, size), "sample_logits")
 
 
+_INT32 = np.dtype(np.int32)
+
+
 def _page_list(a):
     """Page or row numbers on the host as int32; what int32 does not hold is refused, not cut to it."""
-    given = np.asarray(a)
+    given = np.ascontiguousarray(a)
+    if given.dtype == _INT32:  # (the comparison below would add 2 us to a copy of 6)
+        return given
     with np.errstate(invalid="ignore"):
-        out = np.ascontiguousarray(given, np.int32)
-    if given.dtype != np.int32 and not np.array_equal(out, given):
+        out = given.astype(np.int32)
+    if not np.array_equal(out, given):
         raise ValueError("page and token numbers are whole numbers of 32 bits")
     return out
 
