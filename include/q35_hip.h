@@ -48,8 +48,10 @@ typedef struct q35_context q35_context;
 
 /* ------------------------------------------------------------- context
  * Replaces the executor (include/qwen35x/cpu/executor.h:45-123): the GPU grid
- * and one HIP stream take its role. stream == NULL creates a private stream;
- * otherwise the given hipStream_t is used and not destroyed. */
+ * and one HIP stream take its role. stream == NULL creates a private stream (one
+ * that the default stream does not wait for); otherwise the given hipStream_t is
+ * used and not destroyed. The default stream itself, whose handle is NULL too,
+ * cannot be given. */
 int q35_context_create(int device, void *stream, q35_context **out);
 void q35_context_destroy(q35_context *ctx);
 int q35_context_synchronize(q35_context *ctx);
@@ -180,7 +182,7 @@ int q35_attention_decode_paged(q35_context *ctx, const float *q, const float *ga
  * sigmoid(gate); a node that sees nothing, or whose scores are all -inf, gets
  * zero. Infinite or NaN keys and values reach only the nodes that see their
  * row (a key, or a context row's value, that is not finite may leave NaN in
- * those). Scores have to fit fp32, in units of binades.
+ * those). scale q.k times log2(e) has to fit fp32.
  *   head_dim 64, 128 or 256; heads a multiple of kv_heads; page_tokens a power
  *   of two; at most 256 nodes a request; FP16 pools of total_pages pages;
  *   16-byte aligned buffers; pools, table and masks are not written.
