@@ -2,10 +2,10 @@
 // copies before a shared page is written), and the rows of accepted tree nodes
 // moved up behind their request's context. Each copied byte is read once and
 // written once; what bounds the large ones is HBM, the small ones the launch:
-// 2047 pages in 8 layers of 4 KV heads of 256 take 463 us (2.1 GB, 4.6 TB/s read
+// 2047 pages in 8 layers of 4 KV heads of 256 take 460 us (2.1 GB, 4.7 TB/s read
 // and written; a plain copy of 2 GiB reaches 4.9), 8 partly filled pages in 6
-// layers of 2 KV heads 5.2 us (the kernel 3.3), the accepted rows of 64 requests
-// in 6 such layers 5.3 us.
+// layers of 2 KV heads 5.2 to 6.1 us by the host (the kernel 2.7), the accepted
+// rows of 64 requests in 6 such layers 5.3 us.
 #include <algorithm>
 
 #include "q35_device.h"

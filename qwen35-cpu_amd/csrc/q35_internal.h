@@ -534,7 +534,8 @@ struct PageCopyArgs {
 };
 // Pairs of pages, in the kernel's arguments: 256 per launch are 3 KiB; up to 16 go
 // in a launch of their own kind, whose arguments the host hands over sooner (8
-// pages 5.2 against 6.2 us a call, 17 against 24 us where each call is waited for).
+// pages 5.2 against 6.2 us a call on one host, 17 against 24 us where each call is
+// waited for).
 constexpr int kCopyPairs = 256, kFewCopyPairs = 16;
 template <int N>
 struct PagePairsOf {

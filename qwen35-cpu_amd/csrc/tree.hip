@@ -12,16 +12,17 @@
 // probabilities enter the products as two binary16 operands, which doubles the
 // matrix work and keeps the error at that of fp32 sums (3e-7). Measured, heads
 // of 256:
-//   1 request, 611 rows of context, 5 nodes, 8 / 2 heads: 15.7 us, latency: 11
+//   1 request, 611 rows of context, 5 nodes, 8 / 2 heads: 15.8 us, latency: 11
 //     in the attention (as long without its products), 5 in the merge;
-//   16 requests of 64 to 4096 rows, 8 to 16 nodes: 33 us, 28 of them in the
+//   16 requests of 64 to 4096 rows, 8 to 16 nodes: 32.5 us, 27 of them in the
 //     attention (73 MB, 15 us at a large copy's rate; 29 without the products);
 //   64 requests of 1 to 8192 rows, 1 to 23 nodes, 16 / 4 heads: 302 us, 3.7 TB/s
 //     of cache rows (1.1 GB, 220 us at a large copy's rate): loads alone take
 //     248 us and products alone 243, and they overlap but for a fifth;
-//   1 request of 100003 rows, 64 nodes, 16 / 4 heads: 242 us, 434 TFLOP/s of the
-//     formula's, 870 of the matrix units (a large product reaches 1270); loads
-//     alone take 128 us.
+//   1 request of 100003 rows, 64 nodes, 16 / 4 heads: 235 to 242 us, 440 TFLOP/s
+//     of the formula's, 880 of the matrix units (a large product reaches 1270);
+//     matrix units and LDS are each busy for 45% of the cycles; loads alone take
+//     128 us.
 #include <algorithm>
 
 #include "q35_device.h"
